@@ -87,7 +87,8 @@ enum WsSlot {
 constexpr int kMaxHostPanels = 16;
 
 // Kernel classes timed by the optional per-handle profiler (CUDA events on the handle's stream).
-enum ProfKind { kProfTcGemm = 0, kProfFp32Gemm, kProfSplit, kProfScan, kProfRho, kProfReduce, kProfCount };
+enum ProfKind { kProfTcGemm = 0, kProfFp32Gemm, kProfSplit, kProfScan, kProfRho, kProfReduce, kProfQ4, kProfExpert,
+                kProfCount };
 
 struct ProfRec { void* a; void* b; int kind; };   // cudaEvent_t pair
 
@@ -283,5 +284,42 @@ int launch_reduce_f64(const double* P, int G, int M, int N, long ldp, float* C, 
 size_t rho_ws_bytes(int M, int N, long K, int P, int sms);
 int launch_rho(const float* A, long lda, const float* B, long ldb, int M, int N, long K, int P, void* ws, int sms,
                double* out2, void* stream);
+
+// ---------------------------------------------------------------------------------------------------
+// 4-bit weights and expert routing (entry points: q4_expert.cpp)
+constexpr int kMaxExperts = 1024;   // per-expert counters of the sort in shared memory
+
+// k_q4.cu. The packed layout is described in q4_common.cuh.
+size_t q4_bytes(int E, int N, long K, int group);
+int launch_q4_pack(const void* W, long ldw, int dtype, int E, int N, long K, int group, void* packed, int num_sms,
+                   void* stream);
+int launch_q4_unpack(const void* packed, int E, int N, long K, int group, float* W, long ldw, int num_sms, void* stream);
+struct Q4GemmArgs {
+    int R, E, N; long K;               // rows of A and C (with offsets: room for), experts
+    int group, dtype;                  // emu_dtype_t of A and C
+    const void* A; long lda;
+    const void* packed;
+    const int* offsets;                // device, E + 1 row offsets; null: one matrix for all rows
+    void* C; long ldc;
+    int num_sms;
+};
+int launch_q4_rows(const Q4GemmArgs& a, void* stream);   // few rows (per expert)
+
+// k_expert.cu
+struct ExpertRows {
+    long T; int topk; long H;          // tokens, choices per token, row length
+    const int* place;                  // T x topk rows of the sorted matrices
+    const float* w;                    // T x topk, null: 1
+    float* dw;
+    const void* X; long ldx;           // per-token input (X, or dY)
+    const void* S; long lds;           // sorted input
+    void* DS; long ldds;               // sorted output
+    void* Y; long ldy;                 // per-token output
+    int num_sms;
+};
+int launch_expert_sort(const int* expert, int S, int E, int* order, int* place, int* offsets, void* stream);
+int launch_expert_gather(const ExpertRows& a, int dtype, void* stream);
+int launch_expert_combine(const ExpertRows& a, int dtype, void* stream);
+int launch_expert_combine_bwd(const ExpertRows& a, int dtype, void* stream);
 
 }  // namespace emu

@@ -1,0 +1,181 @@
+// q4_expert.cpp - C entry points of the 4-bit weight products and of the expert routing around them: argument checks
+// and dispatch. The kernels are in k_q4.cu and k_expert.cu.
+#include "emugemm_internal.h"
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace emu {
+namespace {
+
+int dtype_size(int dtype) {
+    return dtype == EMU_DTYPE_F32 ? 4 : dtype == EMU_DTYPE_F16 || dtype == EMU_DTYPE_BF16 ? 2 : 0;
+}
+bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
+// a pointer the kernels may access with its element's (or the packed layout's) alignment
+bool bad_ptr(const void* p, int align) { return !p || (reinterpret_cast<uintptr_t>(p) & (align - 1)); }
+
+// Sizes of packed weights: E experts of N x K (K below 2^31, all code bytes addressable)
+bool q4_size_ok(int E, int N, long K) {
+    return E >= 1 && E <= kMaxExperts && N >= 1 && N <= (1 << 30) && K >= 1 && K <= (1L << 30);
+}
+// Sizes of the routing calls: at most 2^30 slots
+bool slots_ok(long T, int topk) { return T >= 0 && topk >= 1 && (T == 0 || topk <= (1L << 30) / T); }
+
+emugemm_status_t q4_product(emugemm_handle_t handle, int R, int E, int N, long K, const void* A, long lda, int dtype,
+                            const int* offsets, bool experts, const void* packed, int group, void* C, long ldc) {
+    Handle* h = reinterpret_cast<Handle*>(handle);
+    if (!h) return EMUGEMM_STATUS_INVALID_HANDLE;
+    const int size = dtype_size(dtype);
+    if (!size || !group_ok(group)) return EMUGEMM_STATUS_INVALID_VALUE;
+    if (R < 0 || R > (1 << 30) || !q4_size_ok(E, N, K) || lda < K || ldc < N) return EMUGEMM_STATUS_INVALID_SIZE;
+    if (R == 0) return EMUGEMM_STATUS_SUCCESS;
+    if (bad_ptr(A, size) || bad_ptr(C, size) || bad_ptr(packed, 16) || (experts && bad_ptr(offsets, 4)))
+        return EMUGEMM_STATUS_INVALID_POINTER;
+    DeviceGuard g(h->device);
+    if (!g.ok) return EMUGEMM_STATUS_INTERNAL_ERROR;
+    Q4GemmArgs a{};
+    a.R = R; a.E = E; a.N = N; a.K = K; a.group = group; a.dtype = dtype;
+    a.A = A; a.lda = lda; a.C = C; a.ldc = ldc;
+    a.packed = packed;
+    a.offsets = experts ? offsets : nullptr;
+    a.num_sms = h->num_sms;
+    ProfScope ps(h, kProfQ4);
+    return from_cuda(launch_q4_rows(a, h->stream));
+}
+
+emugemm_status_t rows_checked(Handle* h, int T, int topk, int H, int dtype, long ld1, long ld2, long ld3) {
+    if (!h) return EMUGEMM_STATUS_INVALID_HANDLE;
+    if (!dtype_size(dtype)) return EMUGEMM_STATUS_INVALID_VALUE;
+    if (!slots_ok(T, topk) || H < 0 || H > (1 << 30) || ld1 < H || ld2 < H || ld3 < H) return EMUGEMM_STATUS_INVALID_SIZE;
+    return EMUGEMM_STATUS_SUCCESS;
+}
+
+emugemm_status_t combine(emugemm_handle_t handle, int T, int topk, int H, const void* S, long lds, int dtype,
+                         const int* place, const float* w, bool weighted, void* Y, long ldy) {
+    Handle* h = reinterpret_cast<Handle*>(handle);
+    emugemm_status_t s = rows_checked(h, T, topk, H, dtype, lds, ldy, ldy);
+    if (s != EMUGEMM_STATUS_SUCCESS || T == 0 || H == 0) return s;
+    const int size = dtype_size(dtype);
+    if (bad_ptr(S, size) || bad_ptr(Y, size) || bad_ptr(place, 4) || (weighted && bad_ptr(w, 4)))
+        return EMUGEMM_STATUS_INVALID_POINTER;
+    DeviceGuard g(h->device);
+    if (!g.ok) return EMUGEMM_STATUS_INTERNAL_ERROR;
+    ExpertRows a{};
+    a.T = T; a.topk = topk; a.H = H; a.num_sms = h->num_sms;
+    a.S = S; a.lds = lds; a.Y = Y; a.ldy = ldy;
+    a.place = place; a.w = weighted ? w : nullptr;
+    ProfScope ps(h, kProfExpert);
+    return from_cuda(launch_expert_combine(a, dtype, h->stream));
+}
+
+}  // namespace
+}  // namespace emu
+
+using emu::Handle;
+
+extern "C" {
+
+size_t emugemm_q4_bytes(int E, int N, long K, int group) {
+    return emu::group_ok(group) && emu::q4_size_ok(E, N, K) ? emu::q4_bytes(E, N, K, group) : 0;
+}
+
+emugemm_status_t emugemm_q4_pack(emugemm_handle_t handle, int E, int N, long K, const void* W, long ldw, int dtype,
+                                 int group, void* packed) {
+    Handle* h = reinterpret_cast<Handle*>(handle);
+    if (!h) return EMUGEMM_STATUS_INVALID_HANDLE;
+    const int size = emu::dtype_size(dtype);
+    if (!size || !emu::group_ok(group)) return EMUGEMM_STATUS_INVALID_VALUE;
+    if (!emu::q4_size_ok(E, N, K) || ldw < K) return EMUGEMM_STATUS_INVALID_SIZE;
+    if (emu::bad_ptr(W, size) || emu::bad_ptr(packed, 16)) return EMUGEMM_STATUS_INVALID_POINTER;
+    emu::DeviceGuard g(h->device);
+    if (!g.ok) return EMUGEMM_STATUS_INTERNAL_ERROR;
+    emu::ProfScope ps(h, emu::kProfQ4);
+    return emu::from_cuda(emu::launch_q4_pack(W, ldw, dtype, E, N, K, group, packed, h->num_sms, h->stream));
+}
+
+emugemm_status_t emugemm_q4_unpack(emugemm_handle_t handle, int E, int N, long K, int group, const void* packed, float* W,
+                                   long ldw) {
+    Handle* h = reinterpret_cast<Handle*>(handle);
+    if (!h) return EMUGEMM_STATUS_INVALID_HANDLE;
+    if (!emu::group_ok(group)) return EMUGEMM_STATUS_INVALID_VALUE;
+    if (!emu::q4_size_ok(E, N, K) || ldw < K) return EMUGEMM_STATUS_INVALID_SIZE;
+    if (emu::bad_ptr(W, 4) || emu::bad_ptr(packed, 16)) return EMUGEMM_STATUS_INVALID_POINTER;
+    emu::DeviceGuard g(h->device);
+    if (!g.ok) return EMUGEMM_STATUS_INTERNAL_ERROR;
+    emu::ProfScope ps(h, emu::kProfQ4);
+    return emu::from_cuda(emu::launch_q4_unpack(packed, E, N, K, group, W, ldw, h->num_sms, h->stream));
+}
+
+emugemm_status_t emugemm_q4_gemm(emugemm_handle_t handle, int M, int N, long K, const void* A, long lda, int dtype,
+                                 const void* packed, int group, void* C, long ldc) {
+    return emu::q4_product(handle, M, 1, N, K, A, lda, dtype, nullptr, false, packed, group, C, ldc);
+}
+
+emugemm_status_t emugemm_q4_gemm_experts(emugemm_handle_t handle, int R, int E, int N, long K, const void* A, long lda,
+                                         int dtype, const int* offsets, const void* packed, int group, void* C,
+                                         long ldc) {
+    return emu::q4_product(handle, R, E, N, K, A, lda, dtype, offsets, true, packed, group, C, ldc);
+}
+
+emugemm_status_t emugemm_expert_sort(emugemm_handle_t handle, int T, int topk, int E, const int* expert, int* order,
+                                     int* place, int* offsets) {
+    Handle* h = reinterpret_cast<Handle*>(handle);
+    if (!h) return EMUGEMM_STATUS_INVALID_HANDLE;
+    if (!emu::slots_ok(T, topk) || E < 1 || E > emu::kMaxExperts) return EMUGEMM_STATUS_INVALID_SIZE;
+    if (emu::bad_ptr(offsets, 4) || (T > 0 && (emu::bad_ptr(expert, 4) || emu::bad_ptr(order, 4) || emu::bad_ptr(place, 4))))
+        return EMUGEMM_STATUS_INVALID_POINTER;
+    emu::DeviceGuard g(h->device);
+    if (!g.ok) return EMUGEMM_STATUS_INTERNAL_ERROR;
+    emu::ProfScope ps(h, emu::kProfExpert);
+    return emu::from_cuda(emu::launch_expert_sort(expert, T * topk, E, order, place, offsets, h->stream));
+}
+
+emugemm_status_t emugemm_expert_gather(emugemm_handle_t handle, int T, int topk, int H, const void* X, long ldx, int dtype,
+                                       const int* place, void* XS, long ldxs) {
+    Handle* h = reinterpret_cast<Handle*>(handle);
+    emugemm_status_t s = emu::rows_checked(h, T, topk, H, dtype, ldx, ldxs, ldxs);
+    if (s != EMUGEMM_STATUS_SUCCESS || T == 0 || H == 0) return s;
+    const int size = emu::dtype_size(dtype);
+    if (emu::bad_ptr(X, size) || emu::bad_ptr(XS, size) || emu::bad_ptr(place, 4)) return EMUGEMM_STATUS_INVALID_POINTER;
+    emu::DeviceGuard g(h->device);
+    if (!g.ok) return EMUGEMM_STATUS_INTERNAL_ERROR;
+    emu::ExpertRows a{};
+    a.T = T; a.topk = topk; a.H = H; a.num_sms = h->num_sms;
+    a.X = X; a.ldx = ldx; a.DS = XS; a.ldds = ldxs; a.place = place;
+    emu::ProfScope ps(h, emu::kProfExpert);
+    return emu::from_cuda(emu::launch_expert_gather(a, dtype, h->stream));
+}
+
+emugemm_status_t emugemm_expert_gather_backward(emugemm_handle_t handle, int T, int topk, int H, const void* dXS,
+                                                long lddxs, int dtype, const int* place, void* dX, long lddx) {
+    return emu::combine(handle, T, topk, H, dXS, lddxs, dtype, place, nullptr, false, dX, lddx);
+}
+
+emugemm_status_t emugemm_expert_combine(emugemm_handle_t handle, int T, int topk, int H, const void* YS, long ldys,
+                                        int dtype, const int* place, const float* weights, void* Y, long ldy) {
+    return emu::combine(handle, T, topk, H, YS, ldys, dtype, place, weights, true, Y, ldy);
+}
+
+emugemm_status_t emugemm_expert_combine_backward(emugemm_handle_t handle, int T, int topk, int H, const void* dY,
+                                                 long lddy, const void* YS, long ldys, int dtype, const int* place,
+                                                 const float* weights, void* dYS, long lddys, float* dweights) {
+    Handle* h = reinterpret_cast<Handle*>(handle);
+    emugemm_status_t s = emu::rows_checked(h, T, topk, H, dtype, lddy, ldys, lddys);
+    if (s != EMUGEMM_STATUS_SUCCESS || T == 0) return s;
+    const int size = emu::dtype_size(dtype);
+    if (emu::bad_ptr(place, 4) || emu::bad_ptr(weights, 4) || emu::bad_ptr(dweights, 4) ||
+        (H > 0 && (emu::bad_ptr(dY, size) || emu::bad_ptr(YS, size) || emu::bad_ptr(dYS, size))))
+        return EMUGEMM_STATUS_INVALID_POINTER;
+    emu::DeviceGuard g(h->device);
+    if (!g.ok) return EMUGEMM_STATUS_INTERNAL_ERROR;
+    emu::ExpertRows a{};
+    a.T = T; a.topk = topk; a.H = H; a.num_sms = h->num_sms;
+    a.X = dY; a.ldx = lddy; a.S = YS; a.lds = ldys; a.DS = dYS; a.ldds = lddys;
+    a.place = place; a.w = weights; a.dw = dweights;
+    emu::ProfScope ps(h, emu::kProfExpert);
+    return emu::from_cuda(emu::launch_expert_combine_bwd(a, dtype, h->stream));
+}
+
+}  // extern "C"

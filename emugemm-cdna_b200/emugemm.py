@@ -24,6 +24,10 @@ SCHEME_NAMES = ["AUTO", "NATIVE_FP32", "FP32_CHUNKED", "BF16X3", "FP16X3", "BF16
 ATTR_TC_KERNEL, ATTR_TC_SPLITK, ATTR_FP32_TILE, ATTR_ROWS_PANELS, ATTR_COMM_SMS, ATTR_BCAST_NCCL = 0, 1, 2, 3, 4, 5
 TC_KERNEL_CODES = {"auto": 0, "single": 1, "pair": 2, "fused": 3, "fusea": 4}
 
+# emu_dtype_t: element types of the 4-bit weight products and of the routed rows
+F32, F16, BF16 = 0, 1, 2
+DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+
 STATUS = {
     0: "SUCCESS", 1: "INVALID_HANDLE", 2: "NOT_IMPLEMENTED", 3: "INVALID_POINTER", 4: "INVALID_SIZE",
     5: "MEMORY_ERROR", 6: "INTERNAL_ERROR", 11: "INVALID_VALUE", 100: "ARCH_MISMATCH", 101: "TIMEOUT",
@@ -121,6 +125,22 @@ _SIGS = {
     "emugemm_sgemm_ksplit": (c_int, [c_void_p, c_int, c_int, c_long, c_void_p, c_long, c_void_p, c_long, c_void_p,
                                      c_long, c_int, c_int, c_int]),
     "emugemm_rows_panels": (c_int, [c_int, c_int, c_int, c_long, c_int, c_int, c_void_p, c_void_p, c_int]),
+    "emugemm_q4_bytes": (c_size_t, [c_int, c_int, c_long, c_int]),
+    "emugemm_q4_pack": (c_int, [c_void_p, c_int, c_int, c_long, c_void_p, c_long, c_int, c_int, c_void_p]),
+    "emugemm_q4_unpack": (c_int, [c_void_p, c_int, c_int, c_long, c_int, c_void_p, c_void_p, c_long]),
+    "emugemm_q4_gemm": (c_int, [c_void_p, c_int, c_int, c_long, c_void_p, c_long, c_int, c_void_p, c_int, c_void_p,
+                                c_long]),
+    "emugemm_q4_gemm_experts": (c_int, [c_void_p, c_int, c_int, c_int, c_long, c_void_p, c_long, c_int, c_void_p,
+                                        c_void_p, c_int, c_void_p, c_long]),
+    "emugemm_expert_sort": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "emugemm_expert_gather": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_long, c_int, c_void_p, c_void_p,
+                                      c_long]),
+    "emugemm_expert_gather_backward": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_long, c_int, c_void_p,
+                                               c_void_p, c_long]),
+    "emugemm_expert_combine": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_long, c_int, c_void_p, c_void_p,
+                                       c_void_p, c_long]),
+    "emugemm_expert_combine_backward": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_long, c_void_p, c_long, c_int,
+                                                c_void_p, c_void_p, c_void_p, c_long, c_void_p]),
     "emugemm_kernel_launch_count": (ctypes.c_ulonglong, []),
     "emugemm_profile_begin": (c_int, [c_void_p]),
     "emugemm_profile_end": (c_int, [c_void_p, P(c_double), P(c_int), c_int]),
@@ -159,6 +179,40 @@ def _ptr(x) -> int:
     if isinstance(x, int):
         return x
     return int(x.data_ptr())
+
+
+_dtype_codes: dict = {}   # tensor dtype -> emu_dtype_t
+
+
+def _dtype(dtype, *xs) -> int:
+    """emu_dtype_t of the operands: the given code, or that of the tensors, which must agree (ValueError)."""
+    for x in xs:
+        d = getattr(x, "dtype", None)
+        if d is None:
+            continue
+        code = _dtype_codes.get(d)
+        if code is None:
+            code = _dtype_codes[d] = DTYPES.get(str(d), -1)
+        if dtype is None:
+            dtype = code
+        elif dtype != code:
+            raise ValueError(f"operands of different types: {d} against {dtype}")
+    if dtype is None:
+        raise ValueError("raw pointers need a dtype (emugemm.F32, F16 or BF16)")
+    return dtype
+
+
+def _typed(x, name: str) -> int:
+    """Pointer of x, which, if a tensor, must have the dtype `name` (ValueError)."""
+    d = getattr(x, "dtype", None)
+    if d is not None and str(d) != name:
+        raise ValueError(f"expected a {name} tensor, got {d}")
+    return _ptr(x)
+
+
+def q4_bytes(E: int, N: int, K: int, group: int) -> int:
+    """Bytes of the packed 4-bit weights of E experts of N x K (emugemm_q4_bytes); 0 when a size is out of range."""
+    return int(lib().emugemm_q4_bytes(E, N, K, group))
 
 
 def check(fn: str, code: int) -> None:
@@ -353,7 +407,61 @@ class Handle:
     def split_f16(self, X, n, hi, lo) -> None:
         check("emugemm_split_f16", lib().emugemm_split_f16(self.h, _ptr(X), n, _ptr(hi), _ptr(lo)))
 
-    PROF_KINDS = ["tc_gemm", "fp32_gemm", "split", "scan", "rho", "reduce"]
+    # ---- 4-bit weights and expert routing (dtype: from the tensors, or emugemm.F32 / F16 / BF16 for raw pointers) ----
+    def q4_pack(self, E, N, K, W, ldw, group, packed, dtype=None) -> None:
+        """Quantise E * N rows of K weights into `packed` (q4_bytes(E, N, K, group) bytes)."""
+        check("emugemm_q4_pack", lib().emugemm_q4_pack(self.h, E, N, K, _ptr(W), ldw, _dtype(dtype, W), group,
+                                                       _ptr(packed)))
+
+    def q4_unpack(self, E, N, K, group, packed, W, ldw) -> None:
+        """The FP32 values of packed weights."""
+        check("emugemm_q4_unpack", lib().emugemm_q4_unpack(self.h, E, N, K, group, _ptr(packed),
+                                                           _typed(W, "torch.float32"), ldw))
+
+    def q4_gemm(self, M, N, K, A, lda, packed, group, C, ldc, dtype=None) -> None:
+        """C (M x N) = A (M x K) * W^T with packed 4-bit weights."""
+        check("emugemm_q4_gemm", lib().emugemm_q4_gemm(self.h, M, N, K, _ptr(A), lda, _dtype(dtype, A, C), _ptr(packed),
+                                                       group, _ptr(C), ldc))
+
+    def q4_gemm_experts(self, R, E, N, K, A, lda, offsets, packed, group, C, ldc, dtype=None) -> None:
+        """q4_gemm with weights of E experts over rows sorted by expert (offsets: E + 1 int32 on the device)."""
+        check("emugemm_q4_gemm_experts",
+              lib().emugemm_q4_gemm_experts(self.h, R, E, N, K, _ptr(A), lda, _dtype(dtype, A, C),
+                                            _typed(offsets, "torch.int32"), _ptr(packed), group, _ptr(C), ldc))
+
+    def expert_sort(self, T, topk, E, expert, order, place, offsets) -> None:
+        """Stable sort of T x topk expert ids; all arrays int32."""
+        i = "torch.int32"
+        check("emugemm_expert_sort", lib().emugemm_expert_sort(self.h, T, topk, E, _typed(expert, i), _typed(order, i),
+                                                               _typed(place, i), _typed(offsets, i)))
+
+    def expert_gather(self, T, topk, H, X, ldx, place, XS, ldxs, dtype=None) -> None:
+        """XS[place[t, j]] = X[t]."""
+        check("emugemm_expert_gather", lib().emugemm_expert_gather(self.h, T, topk, H, _ptr(X), ldx, _dtype(dtype, X, XS),
+                                                                   _typed(place, "torch.int32"), _ptr(XS), ldxs))
+
+    def expert_gather_backward(self, T, topk, H, dXS, lddxs, place, dX, lddx, dtype=None) -> None:
+        """dX[t] = sum over j of dXS[place[t, j]]."""
+        check("emugemm_expert_gather_backward",
+              lib().emugemm_expert_gather_backward(self.h, T, topk, H, _ptr(dXS), lddxs, _dtype(dtype, dXS, dX),
+                                                   _typed(place, "torch.int32"), _ptr(dX), lddx))
+
+    def expert_combine(self, T, topk, H, YS, ldys, place, weights, Y, ldy, dtype=None) -> None:
+        """Y[t] = sum over j of weights[t, j] * YS[place[t, j]] (weights float32)."""
+        check("emugemm_expert_combine",
+              lib().emugemm_expert_combine(self.h, T, topk, H, _ptr(YS), ldys, _dtype(dtype, YS, Y),
+                                           _typed(place, "torch.int32"), _typed(weights, "torch.float32"), _ptr(Y), ldy))
+
+    def expert_combine_backward(self, T, topk, H, dY, lddy, YS, ldys, place, weights, dYS, lddys, dweights,
+                                dtype=None) -> None:
+        """dYS[place[t, j]] = weights[t, j] * dY[t] and dweights[t, j] = <dY[t], YS[place[t, j]]>."""
+        f = "torch.float32"
+        check("emugemm_expert_combine_backward",
+              lib().emugemm_expert_combine_backward(self.h, T, topk, H, _ptr(dY), lddy, _ptr(YS), ldys,
+                                                    _dtype(dtype, dY, YS, dYS), _typed(place, "torch.int32"),
+                                                    _typed(weights, f), _ptr(dYS), lddys, _typed(dweights, f)))
+
+    PROF_KINDS = ["tc_gemm", "fp32_gemm", "split", "scan", "rho", "reduce", "q4", "expert"]
 
     def profile_begin(self) -> None:
         check("emugemm_profile_begin", lib().emugemm_profile_begin(self.h))

@@ -219,7 +219,7 @@ int emugemm_fp32_groups(int M, int N, long K, int chunks, int num_sms);
 
 /* Per-handle kernel timing with CUDA events recorded on the handle's stream around each kernel class:
    0 tensor-core GEMM, 1 FP32 GEMM (+ FP64 reduce), 2 slice split, 3 absmax / exponent scans, 4 rho probe,
-   5 FP64 reduce. profile_end synchronises and returns the summed milliseconds and launch counts of the
+   5 FP64 reduce, 6 4-bit weights, 7 expert routing. profile_end synchronises and returns the summed milliseconds and launch counts of the
    first nkinds classes. */
 emugemm_status_t emugemm_profile_begin(emugemm_handle_t handle);
 emugemm_status_t emugemm_profile_end(emugemm_handle_t handle, double* ms_by_kind, int* count_by_kind,
@@ -282,6 +282,67 @@ int emugemm_fp32_groups_tile(int M, int N, long K, int chunks, int num_sms, int 
    flight land before it exits, and its output is not meaningful. emugemm_sync (or emugemm_noalloc_sync) then
    returns EMUGEMM_STATUS_TIMEOUT. No fault, trap or hang is involved; n = 0 cancels. */
 void emugemm_test_stall_next_launches(int n);
+
+/* ---- 4-bit weights and expert routing (no emugemm-cdna counterpart) ----------------------------------------------
+   Products whose weights are held in 4 bits, for one token up to a prompt, and the row movements that send tokens to
+   experts with weights of their own and back. All matrices are row-major device buffers of the handle's device; A, C
+   and the routed rows are FP32, FP16 or BF16 (emu_dtype_t, the same type in and out), every leading dimension counts
+   elements and may exceed the row length, inputs and outputs must not overlap. The calls are asynchronous on the
+   handle's stream, allocate nothing and can be captured into CUDA graphs. Sums are FP32 in a fixed order (no atomics):
+   the same call gives the same bits. Status: INVALID_VALUE for an unknown dtype or group, INVALID_SIZE for a size or
+   leading dimension out of range, INVALID_POINTER for a null or misaligned pointer (elements by their size, packed
+   weights by 16 bytes). Device-side indices (offsets, place) are bounds-checked by the kernels: a bad one touches no
+   memory outside the given matrices. */
+typedef enum { EMU_DTYPE_F32 = 0, EMU_DTYPE_F16 = 1, EMU_DTYPE_BF16 = 2 } emu_dtype_t;
+
+/* Bytes of the packed weights of E experts (1 for a plain matrix; at most 1024) of N x K, with one scale per `group`
+   (32, 64 or 128) values along K; the last group of a row may be shorter. 0 when a size is out of range. Layout (a
+   program may also write it itself, from weights quantised elsewhere to q = -8..7 and bf16 scales):
+     codes: q + 8 (8 = zero in the padding), N padded to 16 rows and K to 64; tiles of 16 rows x 64 values of K of 512
+       bytes, ordered [expert][row block][k block]; bytes (4g + t) * 16 .. + 15 of a tile (g = 0..7, t = 0..3) are four
+       32-bit words: row g at k = 8t..8t+7, row g + 8 at the same k, row g at k = 32 + 8t.., row g + 8 at the same; in a
+       word k = 0, 2, 4, 6, 1, 3, 5, 7 take the nibbles from the lowest up;
+     scales: at the next multiple of 256 bytes, bf16 [expert][row block][group][8][2], rows g and g + 8 side by side. */
+size_t emugemm_q4_bytes(int E, int N, long K, int group);
+/* Quantises W (E * N rows of K values, ldw >= K; a linear layer's weights, one row per output) into `packed`. Per group
+   scale = bf16(fp32(max|w| / 7)), q = w / scale rounded to the nearest integer (ties to even, decided exactly) and kept
+   within -7..7. A group of zeros, or so small that the scale rounds to 0, reads as zeros; a group that holds NaN or Inf
+   reads as NaN. */
+emugemm_status_t emugemm_q4_pack(emugemm_handle_t handle, int E, int N, long K, const void* W, long ldw, int dtype,
+                                 int group, void* packed);
+/* The FP32 values scale * q (exact) of packed weights: E * N rows of K, ldw >= K. */
+emugemm_status_t emugemm_q4_unpack(emugemm_handle_t handle, int E, int N, long K, int group, const void* packed, float* W,
+                                   long ldw);
+/* C (M x N) = A (M x K) * W^T with packed weights W (N x K): sum over the groups of scale * (sum over the group of
+   q * a), all products exact, sums in FP32, rounded once to C's type. Magnitudes of A above about 3e35 can overflow a
+   group's sum. FP32 A is taken as three bf16 slices: exact above 2^-110 in magnitude, low bits dropped below. */
+emugemm_status_t emugemm_q4_gemm(emugemm_handle_t handle, int M, int N, long K, const void* A, long lda, int dtype,
+                                 const void* packed, int group, void* C, long ldc);
+/* The same with weights of E experts: rows offsets[e] .. offsets[e+1] - 1 of A and C (device array of E + 1, not
+   decreasing, as made by emugemm_expert_sort) use expert e's weights; the other rows of C, up to R, are left as they
+   were. The work follows the rows that are there, not R. */
+emugemm_status_t emugemm_q4_gemm_experts(emugemm_handle_t handle, int R, int E, int N, long K, const void* A, long lda,
+                                         int dtype, const int* offsets, const void* packed, int group, void* C,
+                                         long ldc);
+/* Stable sort of T x topk expert ids (slot s = token * topk + choice; at most 2^30 slots, E <= 1024): slots of expert e
+   become the rows offsets[e] .. offsets[e+1] - 1, in slot order. place[s] is the slot's row and order[row] its slot; an
+   id outside [0, E) (a dropped or padding token) has no row: place[s] = -1, and order is -1 from offsets[E] on. */
+emugemm_status_t emugemm_expert_sort(emugemm_handle_t handle, int T, int topk, int E, const int* expert, int* order,
+                                     int* place, int* offsets);
+/* XS[place[t, j]] = X[t] (rows of H). Rows of XS that no slot has are left as they were. */
+emugemm_status_t emugemm_expert_gather(emugemm_handle_t handle, int T, int topk, int H, const void* X, long ldx, int dtype,
+                                       const int* place, void* XS, long ldxs);
+/* Gradient of emugemm_expert_gather: dX[t] = sum over j of dXS[place[t, j]]; 0 for a token without an expert. */
+emugemm_status_t emugemm_expert_gather_backward(emugemm_handle_t handle, int T, int topk, int H, const void* dXS,
+                                                long lddxs, int dtype, const int* place, void* dX, long lddx);
+/* Y[t] = sum over j of weights[t, j] * YS[place[t, j]] (weights FP32, T x topk); 0 for a token without an expert. */
+emugemm_status_t emugemm_expert_combine(emugemm_handle_t handle, int T, int topk, int H, const void* YS, long ldys,
+                                        int dtype, const int* place, const float* weights, void* Y, long ldy);
+/* Gradients of emugemm_expert_combine: dYS[place[t, j]] = weights[t, j] * dY[t] (other rows of dYS left as they were)
+   and dweights[t, j] = <dY[t], YS[place[t, j]]> (FP32; 0 for a slot without a row). */
+emugemm_status_t emugemm_expert_combine_backward(emugemm_handle_t handle, int T, int topk, int H, const void* dY,
+                                                 long lddy, const void* YS, long ldys, int dtype, const int* place,
+                                                 const float* weights, void* dYS, long lddys, float* dweights);
 
 /* ---- several GPUs of one node: one process (and one handle) per GPU, NCCL between them ---------------------------
    No emugemm-cdna counterpart (the reference runs on one GPU); these are the two partitioned forms of its benchmark
