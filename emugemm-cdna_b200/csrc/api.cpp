@@ -40,6 +40,7 @@ void* ws_get(Handle* h, int slot, size_t bytes) {
     if (h->ws_size[slot] >= bytes) return h->ws[slot];
     size_t total = 0;
     for (int i = 0; i < kWsCount; ++i) total += (i == slot) ? 0 : h->ws_size[i];
+    for (const Handle::Retired* r = h->retired; r; r = r->next) total += r->bytes;
     if (h->ws_limit && total + bytes > h->ws_limit) return nullptr;
     if (h->ws[slot]) {
         cudaStreamSynchronize((cudaStream_t)h->stream);
@@ -53,6 +54,30 @@ void* ws_get(Handle* h, int slot, size_t bytes) {
     }
     h->ws_size[slot] = bytes;
     return h->ws[slot];
+}
+
+void* ws_get_kept(Handle* h, int slot, size_t bytes) {
+    if (bytes == 0) bytes = 256;
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing((cudaStream_t)h->stream, &cap) != cudaSuccess) {
+        cudaGetLastError();   // the legacy stream while another stream captures: as if capturing
+        cap = cudaStreamCaptureStatusActive;
+    }
+    if (cap != cudaStreamCaptureStatusNone) {
+        if (h->ws_size[slot] < bytes) return nullptr;
+        h->ws_kept[slot] = true;
+        return h->ws[slot];
+    }
+    if (h->ws_size[slot] < bytes && h->ws_kept[slot]) {
+        Handle::Retired* r = (Handle::Retired*)std::malloc(sizeof(Handle::Retired));
+        if (!r) return nullptr;
+        *r = Handle::Retired{h->ws[slot], h->ws_size[slot], h->retired};
+        h->retired = r;
+        h->ws[slot] = nullptr;
+        h->ws_size[slot] = 0;
+        h->ws_kept[slot] = false;
+    }
+    return ws_get(h, slot, bytes);
 }
 
 DeviceGuard::DeviceGuard(int dev) {
@@ -527,6 +552,11 @@ emugemm_status_t emugemm_destroy_handle(emugemm_handle_t handle) {
     emu::multigpu_release(h);
     for (int i = 0; i < emu::kWsCount; ++i)
         if (h->ws[i]) cudaFree(h->ws[i]);
+    while (Handle::Retired* r = h->retired) {
+        h->retired = r->next;
+        cudaFree(r->p);
+        std::free(r);
+    }
     emu::prof_clear(h);
     delete[] h->prof;
     if (h->err_host) cudaFreeHost(h->err_host);

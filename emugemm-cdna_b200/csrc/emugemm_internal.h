@@ -80,6 +80,7 @@ enum WsSlot {
     kWsCommP,                       // emugemm_sgemm_ksplit: the FP64 partial product and its sum over ranks
     // bank 1 of the per-product scratch (Handle::bank), for a second panel GEMM running beside the first
     kWsSplitB0b, kWsSplitB1b, kWsScaleBb, kWsSplitKb, kWsF64Accb,
+    kWsQ4X,                         // q4 products: rows of A as TMA reads them (FP32 slices, unaligned rows)
     kWsCount
 };
 
@@ -99,6 +100,9 @@ struct Handle {
     size_t ws_limit = 0;            // 0 = no cap
     void* ws[kWsCount] = {};
     size_t ws_size[kWsCount] = {};
+    // Slots a captured graph refers to (ws_get_kept): their memory lives as long as the handle.
+    bool ws_kept[kWsCount] = {};
+    struct Retired { void* p; size_t bytes; Retired* next; } * retired = nullptr;
     unsigned* err_host = nullptr;   // mapped pinned word
     unsigned* err_dev = nullptr;
     bool profiling = false;
@@ -151,6 +155,10 @@ struct ProfScope {
 };
 
 void* ws_get(Handle* h, int slot, size_t bytes);
+// ws_get for calls that may be captured into a CUDA graph: while the handle's stream captures, a slot that is too small
+// gives null (nothing may be allocated then), and what a capture was given is never freed or moved before the handle is
+// destroyed: a later call that needs more gets new memory beside it.
+void* ws_get_kept(Handle* h, int slot, size_t bytes);
 void count_launch(unsigned n = 1);
 // Testing hook (emugemm_test_stall_next_launches): true for each of the next n launches of a kernel that has one (the
 // single-CTA tensor-core kernel, the TMA-fed FP32 kernel), which then gives up a 1 ms wait on a barrier nothing
@@ -301,9 +309,14 @@ struct Q4GemmArgs {
     const void* packed;
     const int* offsets;                // device, E + 1 row offsets; null: one matrix for all rows
     void* C; long ldc;
+    void* stage;                       // q4_stage_bytes of workspace for launch_q4_tiles (null when that is 0)
+    unsigned* err;
     int num_sms;
 };
 int launch_q4_rows(const Q4GemmArgs& a, void* stream);   // few rows (per expert)
+// k_q4_tc.cu: many rows
+size_t q4_stage_bytes(const void* A, long lda, int dtype, int R, long K);
+int launch_q4_tiles(const Q4GemmArgs& a, void* stream);
 
 // k_expert.cu
 struct ExpertRows {

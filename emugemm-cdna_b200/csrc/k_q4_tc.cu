@@ -1,0 +1,523 @@
+// k_q4_tc.cu - the product with 4-bit weights for many rows, on CTA pairs (tcgen05, cta_group::2).
+//
+// D (256 weight rows x TN rows of A, in TMEM) += Q (integers of the codes) * A^T: the weights are the MMA's A operand, so
+// a thread of the epilogue owns one weight row and a group's scale is one register. Every scale group gets a fresh
+// accumulator; the epilogue warps add it to FP32 registers times the scale, so no weight is rounded and the tensor
+// cores' truncating accumulation never runs over more than 128 values of K. FP32 A is three bf16 slices (lo, mid, hi
+// multiplied in this order into the same accumulator).
+//
+// Per CTA of a pair: 128 weight rows, TN / 2 rows of A. Four converter warps turn the codes (one 16-byte load is rows g
+// and g + 8 at two 8-value chunks) into the 128-byte-swizzled K-major operand in shared memory, rows of A come by TMA,
+// each CTA's part completing on the leader's barrier. Warps: warpgroup 0 = TMA producer, MMA issuer (leader) / TMEM
+// allocator; 1 = converters; 2-3 = scale, sum and store. Registers per warpgroup with setmaxnreg: 80 / 80 / 176 / 176 of
+// the launch's 512 x 128. The peer's converters report to the leader by 16-byte bulk copies (as in k_tc_fused.cu).
+// All waits are bounded.
+#include "device_utils.cuh"
+#include "q4_common.cuh"
+
+#include <algorithm>
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <type_traits>
+
+namespace emu {
+
+bool tc_get_encode(PFN_cuTensorMapEncodeTiled_v12000* out);
+
+namespace {
+
+using namespace dev;
+using namespace q4;
+
+constexpr int kThreads = 512;
+constexpr int kEpiWarps = 8, kConvWarps = 4;
+constexpr int kRegEpi = 176, kRegOther = 80;
+static_assert(2 * 128 * kRegEpi + 2 * 128 * kRegOther == kThreads * 128, "register split");
+constexpr int kPanelA = 128 * 128;            // bytes of 128 weight rows x 64 values
+constexpr int kMaxStages = 6, kMaxBufs = 4;
+constexpr int kSmemMax = 227 * 1024;
+
+// SL: slices of A's rows (1 or 3); a stage holds PP panels of 64 values of K.
+template <int SL, int TN>
+struct Cfg {
+    static constexpr int PP = SL == 1 ? 2 : 1;
+    static constexpr int PANEL_B = TN / 2 * 128;                  // bytes of one slice, 64 values
+    static constexpr int A_BYTES = PP * kPanelA, B_BYTES = PP * SL * PANEL_B;
+    static constexpr int STAGE = A_BYTES + B_BYTES;
+    static constexpr int FIXED = 1024 + 1024;                     // alignment, barriers
+    static constexpr int STAGES = (kSmemMax - FIXED - (kMaxExperts + 1) * 4) / STAGE < kMaxStages
+                                      ? (kSmemMax - FIXED - (kMaxExperts + 1) * 4) / STAGE : kMaxStages;
+    static constexpr int BUFS = 512 / TN < kMaxBufs ? 512 / TN : kMaxBufs;
+    static constexpr int SMEM = STAGES * STAGE + FIXED + (kMaxExperts + 1) * 4;
+    static_assert(STAGES >= 2 && SMEM <= kSmemMax, "shared memory");
+    static_assert(STAGE % 1024 == 0 && PANEL_B % 1024 == 0, "swizzle atoms");
+};
+
+struct Ctl {
+    uint64_t b_full[kMaxStages];    // leader: the rows of A of both CTAs have landed
+    uint64_t a_full[kMaxStages];    // leader: both CTAs' weights are converted
+    uint64_t empty[kMaxStages];     // both: the leader's commit
+    uint64_t tmem_full[kMaxBufs];   // both: the leader's commit
+    uint64_t tmem_empty[kMaxBufs];  // leader: 2 x 8 epilogue warps
+    uint64_t drain;
+    uint32_t tmem_base;
+    int abort;
+    alignas(16) uint32_t sig_src[4];
+    alignas(16) uint32_t sig_dst[kConvWarps][4];
+};
+static_assert(sizeof(Ctl) <= 1024, "barriers");
+
+struct Params {
+    const uint8_t* packed; Layout l;
+    void* C; long ldc;
+    const int* offsets;             // null: one matrix
+    int R, E, N;
+    int num_n;                      // 256-row tiles of the weights
+    int nst;                        // stages per tile
+    int group;
+    int plane;                      // rows between the slices of A (SL = 3)
+    unsigned* err;
+};
+
+__device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
+    const uint32_t a = smem_u32(bar);
+    const unsigned long long t0 = globaltimer();
+    while (!mbar_try_wait(a, parity))
+        if (globaltimer() - t0 > 200000000ull) return;
+}
+__device__ __forceinline__ void abort_pair(Ctl* ctl, uint32_t peer) {
+    ctl->abort = 1;
+    st_shared_cluster_u32(mapa_shared(smem_u32(&ctl->abort), peer), 1u);
+}
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// The tile's expert, 256-row block of weights, and rows [m0, m1) of A. first[e] is the first row tile of expert e.
+struct Tile { int e, nb, m0, m1; };
+template <int TN>
+__device__ __forceinline__ Tile tile_of(const Params& p, const int* first, int t) {
+    Tile r;
+    r.nb = t % p.num_n;
+    const int mt = t / p.num_n;
+    if (!p.offsets) {
+        r.e = 0;
+        r.m0 = mt * TN;
+        r.m1 = min(p.R, r.m0 + TN);
+        return r;
+    }
+    int lo = 0, hi = p.E;            // first[lo] <= mt < first[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= mt) lo = mid;
+        else hi = mid;
+    }
+    r.e = lo;
+    r.m0 = max(0, p.offsets[lo]) + (mt - first[lo]) * TN;
+    r.m1 = min(min(p.R, p.offsets[lo + 1]), r.m0 + TN);
+    return r;
+}
+
+// T: type of A and C. TN: rows of A per tile of the pair.
+template <typename T, int TN>
+__global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__ CUtensorMap tm_x, Params p) {
+    constexpr bool BF16 = !std::is_same<T, __half>::value;
+    constexpr int SL = sizeof(T) == 4 ? 3 : 1;
+    using C_ = Cfg<SL, TN>;
+    constexpr int PP = C_::PP, ST = C_::STAGES, NB = C_::BUFS;
+    constexpr uint32_t kIdesc = idesc_f16(256, TN, BF16);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Ctl* ctl = reinterpret_cast<Ctl*>(smem + ST * C_::STAGE);
+    int* first = reinterpret_cast<int*>(ctl + 1);
+    volatile int* abort = &ctl->abort;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank(), peer = rank ^ 1u;
+    const bool leader = rank == 0;
+    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(&ctl->b_full[s], 1);
+            mbar_init(&ctl->a_full[s], kConvWarps);
+            mbar_init(&ctl->empty[s], 1);
+        }
+        for (int b = 0; b < NB; ++b) {
+            mbar_init(&ctl->tmem_full[b], 1);
+            mbar_init(&ctl->tmem_empty[b], 2 * kEpiWarps);
+        }
+        mbar_init(&ctl->drain, 1);
+        ctl->abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 0 && lane == 0) prefetch_tmap(&tm_x);
+    if (warp == 1) {
+        tmem_alloc_pair(&ctl->tmem_base, 512);
+        tmem_relinquish_pair();
+    }
+    if (warp == 2 && p.offsets) {
+        int run = 0;
+        for (int x0 = 0; x0 < p.E; x0 += 32) {
+            const int x = x0 + lane;
+            const int rows = x < p.E ? min(p.R, p.offsets[x + 1]) - max(0, p.offsets[x]) : 0;
+            const int n = rows > 0 ? (rows + TN - 1) / TN : 0;
+            int inc = n;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, inc, d);
+                if (lane >= d) inc += v;
+            }
+            if (x < p.E) first[x] = run + inc - n;
+            run += __shfl_sync(0xffffffffu, inc, 31);
+        }
+        if (lane == 0) first[p.E] = run;
+    }
+    tc_fence_before();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = ctl->tmem_base;
+    const int num_tiles = (p.offsets ? first[p.E] : (p.R + TN - 1) / TN) * p.num_n;
+
+    if (warp < 8) {
+        reg_dec<kRegOther>();
+        if (warp == 0 && lane == 0) {
+            // ---------------- TMA producer: this CTA's half of the rows of A ----------------
+            const uint32_t lead_full0 = mapa_shared(smem_u32(&ctl->b_full[0]), 0);
+            long it = 0;
+            bool ok = true;
+            for (int t = pair; t < num_tiles && ok; t += num_pairs) {
+                const Tile tl = tile_of<TN>(p, first, t);
+                const int row = tl.m0 + (int)rank * (TN / 2);
+                for (int kst = 0; kst < p.nst; ++kst, ++it) {
+                    const int s = (int)(it % ST);
+                    if (!mbar_wait_cluster(&ctl->empty[s], (uint32_t)((it / ST) & 1) ^ 1u, abort, p.err,
+                                           kErrTimeoutProducer)) {
+                        ok = false;
+                        break;
+                    }
+                    if (leader) mbar_arrive_expect_tx(&ctl->b_full[s], 2 * C_::B_BYTES);
+                    const uint32_t fb = lead_full0 + (uint32_t)(s * sizeof(uint64_t));
+                    uint8_t* st = smem + s * C_::STAGE + C_::A_BYTES;
+#pragma unroll
+                    for (int pn = 0; pn < PP; ++pn)
+#pragma unroll
+                        for (int sl = 0; sl < SL; ++sl)
+                            tma_load_2d_pair(st + (pn * SL + sl) * C_::PANEL_B, &tm_x, fb, (kst * PP + pn) * 64,
+                                             sl * p.plane + row);
+                }
+            }
+            if (!ok) {
+                abort_pair(ctl, peer);
+                if (leader)
+                    for (long j = it > ST ? it - ST : 0; j < it; ++j)
+                        drain_wait(&ctl->b_full[j % ST], (uint32_t)((j / ST) & 1));
+            }
+        } else if (warp == 1 && lane == 0 && leader) {
+            // ---------------- leader: pair MMA issuer ----------------
+            const int spg = p.group / 16;          // k16 steps per scale group
+            long it = 0, ch = 0;
+            bool ok = true;
+            for (int t = pair; t < num_tiles && ok; t += num_pairs) {
+                int step = 0;
+                for (int kst = 0; kst < p.nst && ok; ++kst, ++it) {
+                    const int s = (int)(it % ST);
+                    const uint32_t ph = (uint32_t)((it / ST) & 1);
+                    if (!mbar_wait_cluster(&ctl->b_full[s], ph, abort, p.err, kErrTimeoutMma) ||
+                        !mbar_wait_cluster(&ctl->a_full[s], ph, abort, p.err, kErrTimeoutMma)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(smem + s * C_::STAGE), sb = sa + C_::A_BYTES;
+                    for (int pn = 0; pn < PP && ok; ++pn) {
+                        const uint64_t a = sdesc_kmajor(sa + pn * kPanelA, 128);
+                        const uint64_t b = sdesc_kmajor(sb + pn * SL * C_::PANEL_B, 128);
+                        for (int ks = 0; ks < 4; ++ks, ++step) {
+                            const int u = (int)(ch % NB);
+                            if (step % spg == 0) {
+                                if (!mbar_wait_cluster(&ctl->tmem_empty[u], (uint32_t)((ch / NB) & 1) ^ 1u, abort, p.err,
+                                                       kErrTimeoutMma)) {
+                                    ok = false;
+                                    break;
+                                }
+                                tc_fence_after();
+                            }
+                            const uint32_t d = tmem_base + (uint32_t)(u * TN);
+                            const uint64_t adv = (uint64_t)(ks * 32) >> 4;
+#pragma unroll
+                            for (int sl = SL - 1; sl >= 0; --sl)
+                                mma_f16_ss_pair(d, a + adv, b + adv + (uint64_t)((sl * C_::PANEL_B) >> 4), kIdesc,
+                                                step % spg != 0 || sl != SL - 1 ? 1u : 0u);
+                            if (step % spg == spg - 1) {
+                                mma_commit_pair_both(&ctl->tmem_full[u], (uint16_t)0x3);
+                                ++ch;
+                            }
+                        }
+                    }
+                    if (!ok) break;
+                    mma_commit_pair_both(&ctl->empty[s], (uint16_t)0x3);
+                }
+            }
+            if (!ok) {
+                abort_pair(ctl, peer);
+                mma_commit_pair(&ctl->drain);
+                drain_wait(&ctl->drain, 0);
+            }
+        } else if (warp >= 4) {
+            // ---------------- converters: codes -> integers in the swizzled K-major operand ----------------
+            const int cw = warp - 4, g = lane >> 2, t4 = lane & 3;
+            const uint32_t lead_full0 = mapa_shared(smem_u32(&ctl->a_full[0]), 0);
+            const uint32_t lead_slot = mapa_shared(smem_u32(&ctl->sig_dst[cw][0]), 0);
+            const uint32_t sig_src = smem_u32(&ctl->sig_src[0]);
+            const uint4 none = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+            const uint4* codes = reinterpret_cast<const uint4*>(p.packed);
+            const bool odd = g & 1;
+            long it = 0;
+            bool ok = true;
+            for (int t = pair; t < num_tiles && ok; t += num_pairs) {
+                const Tile tl = tile_of<TN>(p, first, t);
+                const long rb = (long)tl.nb * 16 + (long)rank * 8 + 2 * cw;   // this warp's two row blocks of 16
+                const uint4* src = codes + (((size_t)tl.e * p.l.nb + rb) * p.l.kb) * 32 + lane;
+                auto load = [&](int kst, uint4 (&c)[2][PP]) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+#pragma unroll
+                        for (int pn = 0; pn < PP; ++pn) {
+                            const long kb = (long)kst * PP + pn;
+                            c[r][pn] = rb + r < p.l.nb && kb < p.l.kb ? __ldg(src + ((size_t)r * p.l.kb + kb) * 32) : none;
+                        }
+                };
+                uint4 next[2][PP];
+                load(0, next);
+                for (int kst = 0; kst < p.nst; ++kst, ++it) {
+                    const int s = (int)(it % ST);
+                    uint4 c[2][PP];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+#pragma unroll
+                        for (int pn = 0; pn < PP; ++pn) c[r][pn] = next[r][pn];
+                    if (kst + 1 < p.nst) load(kst + 1, next);
+                    const bool ready = mbar_wait_cluster(&ctl->empty[s], (uint32_t)((it / ST) & 1) ^ 1u, abort, p.err,
+                                                         kErrTimeoutConvert);
+                    if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
+                    uint8_t* st = smem + s * C_::STAGE;
+#pragma unroll
+                    for (int pn = 0; pn < PP; ++pn)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            // rows g and g + 8, chunks t4 and 4 + t4; odd rows store the upper chunk first, so that the
+                            // eight lanes of a store phase (two rows) touch all eight 16-byte columns
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                const int row = (2 * cw + r) * 16 + g + 8 * half;
+                                const uint32_t lo = half ? c[r][pn].y : c[r][pn].x, hi = half ? c[r][pn].w : c[r][pn].z;
+                                const uint32_t w0 = odd ? hi : lo, w1 = odd ? lo : hi;
+                                const int c0 = odd ? 4 + t4 : t4, c1 = c0 ^ 4;
+                                uint8_t* o = st + pn * kPanelA + row * 128;
+                                uint4 v;
+                                v.x = code_pair<BF16>(w0, 0); v.y = code_pair<BF16>(w0, 1);
+                                v.z = code_pair<BF16>(w0, 2); v.w = code_pair<BF16>(w0, 3);
+                                *reinterpret_cast<uint4*>(o + ((c0 ^ g) << 4)) = v;
+                                v.x = code_pair<BF16>(w1, 0); v.y = code_pair<BF16>(w1, 1);
+                                v.z = code_pair<BF16>(w1, 2); v.w = code_pair<BF16>(w1, 3);
+                                *reinterpret_cast<uint4*>(o + ((c1 ^ g) << 4)) = v;
+                            }
+                        }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (leader) {
+                            if (cw == 0) mbar_arrive_expect_tx(&ctl->a_full[s], 16 * kConvWarps);
+                            else mbar_arrive(&ctl->a_full[s]);
+                        } else {
+                            bulk_signal_cluster(lead_slot, sig_src, 16, lead_full0 + (uint32_t)(s * sizeof(uint64_t)));
+                        }
+                    }
+                }
+            }
+            if (!ok && lane == 0) abort_pair(ctl, peer);
+        }
+    } else {
+        reg_inc<kRegEpi>();
+        // ---------------- scale, sum, store: one weight row and half of the tile's rows of A per thread ----------------
+        const int sp = warp & 3, half = (warp - 8) >> 2;
+        const int row_in_tile = (int)rank * 128 + sp * 32 + lane;
+        const uint32_t lane_off = (uint32_t)(sp * 32) << 16;
+        const uint32_t lead_te0 = mapa_shared(smem_u32(&ctl->tmem_empty[0]), 0);
+        const uint16_t* scales = reinterpret_cast<const uint16_t*>(p.packed + p.l.scales_at);
+        const int groups = p.nst * PP * 64 / p.group;      // of the padded K
+        constexpr int H = TN / 2;
+        long ch = 0;
+        bool ok = true;
+        for (int t = pair; t < num_tiles && ok; t += num_pairs) {
+            const Tile tl = tile_of<TN>(p, first, t);
+            const int n = tl.nb * 256 + row_in_tile;
+            const bool there = n < p.N;
+            const uint16_t* sc = scales + ((size_t)tl.e * p.l.nb + (n >> 4)) * p.l.groups * 16 + (n & 7) * 2 + ((n >> 3) & 1);
+            float sum[H];
+#pragma unroll
+            for (int j = 0; j < H; ++j) sum[j] = 0.f;
+            float s_next = there ? __uint_as_float((uint32_t)__ldg(sc) << 16) : 0.f;
+            for (int gi = 0; gi < groups; ++gi, ++ch) {
+                const int u = (int)(ch % NB);
+                const float s = s_next;
+                s_next = there && gi + 1 < p.l.groups ? __uint_as_float((uint32_t)__ldg(sc + (gi + 1) * 16) << 16) : 0.f;
+                const bool ready = mbar_wait_cluster(&ctl->tmem_full[u], (uint32_t)((ch / NB) & 1), abort, p.err,
+                                                     kErrTimeoutEpilogue);
+                if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t tb = tmem_base + lane_off + (uint32_t)(u * TN + half * H);
+#pragma unroll
+                for (int q = 0; q < H / 16; ++q) {
+                    uint32_t r[16];
+                    tmem_ld_32x32b_x16(tb + (uint32_t)(q * 16), r);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) sum[q * 16 + j] = fmaf(s, __uint_as_float(r[j]), sum[q * 16 + j]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_remote(lead_te0 + (uint32_t)(u * sizeof(uint64_t)));
+            }
+            if (!ok) break;
+            if (there) {
+                T* c = static_cast<T*>(p.C) + (size_t)(tl.m0 + half * H) * p.ldc + n;
+                const int rows = tl.m1 - tl.m0 - half * H;
+#pragma unroll
+                for (int j = 0; j < H; ++j)
+                    if (j < rows) c[(size_t)j * p.ldc] = from_float<T>(sum[j]);
+            }
+        }
+        if (!ok && lane == 0) abort_pair(ctl, peer);
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+// Rows of A as TMA can read them: 16-bit rows of Kp values (zeros behind K), FP32 rows as three planes of bf16 slices.
+template <typename T>
+__global__ void __launch_bounds__(256) k_q4_stage(const T* __restrict__ A, long lda, int R, long K, long Kp,
+                                                  uint16_t* __restrict__ X, int vec) {
+    const long chunks = Kp / 8, n = (long)R * chunks;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
+        const long m = i / chunks, k = (i - m * chunks) * 8;
+        const T* a = A + (size_t)m * lda + k;
+        T x[8];
+        if (sizeof(T) == 4 && vec && k + 8 <= K) {
+            reinterpret_cast<float4*>(x)[0] = reinterpret_cast<const float4*>(a)[0];
+            reinterpret_cast<float4*>(x)[1] = reinterpret_cast<const float4*>(a)[1];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = k + j < K ? a[j] : from_float<T>(0.f);
+        }
+        if (sizeof(T) == 4) {
+            __align__(16) uint16_t s[3][8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) slice3(to_float<T>(x[j]), s[0][j], s[1][j], s[2][j]);
+#pragma unroll
+            for (int q = 0; q < 3; ++q)
+                *reinterpret_cast<uint4*>(X + ((size_t)q * R + m) * Kp + k) = *reinterpret_cast<const uint4*>(s[q]);
+        } else {
+            *reinterpret_cast<uint4*>(X + (size_t)m * Kp + k) = *reinterpret_cast<const uint4*>(x);
+        }
+    }
+}
+
+template <typename T, int TN>
+int launch_pair(const Q4GemmArgs& a, const void* X, long ldx, int rows, long kx, int plane, cudaStream_t st) {
+    constexpr int SL = sizeof(T) == 4 ? 3 : 1;
+    using C_ = Cfg<SL, TN>;
+    PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
+    if (!tc_get_encode(&enc)) return (int)cudaErrorNotSupported;
+    CUtensorMap tm;
+    cuuint64_t dims[2] = {(cuuint64_t)kx, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ldx * 2};
+    cuuint32_t box[2] = {64, (cuuint32_t)(TN / 2)};
+    cuuint32_t estr[2] = {1, 1};
+    if (enc(&tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(X), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return (int)cudaErrorInvalidValue;
+    Params p{};
+    p.packed = static_cast<const uint8_t*>(a.packed);
+    p.l = layout(a.E, a.N, a.K, a.group);
+    p.C = a.C; p.ldc = a.ldc;
+    p.offsets = a.offsets;
+    p.R = a.R; p.E = a.E; p.N = a.N;
+    p.num_n = (a.N + 255) / 256;
+    p.nst = (int)((a.K + 127) / 128 * (2 / C_::PP));
+    p.group = a.group;
+    p.plane = plane;
+    p.err = a.err;
+    auto kern = k_q4_pair<T, TN>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM);
+    if (e != cudaSuccess) return (int)e;
+    // with offsets the number of tiles is known on the device only: at most one partly filled tile per expert
+    const long tiles = ((a.offsets ? std::min(a.E, a.R) : 0) + ((long)a.R + TN - 1) / TN) * p.num_n;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(2 * std::min((long)a.num_sms / 2, tiles)), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = C_::SMEM;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kern, tm, p);
+    count_launch();
+    if (e != cudaSuccess) return (int)e;
+    return (int)cudaGetLastError();
+}
+
+template <typename T>
+int launch_t(const Q4GemmArgs& a, cudaStream_t st) {
+    constexpr int SL = sizeof(T) == 4 ? 3 : 1;
+    const void* X = a.A;
+    long ldx = a.lda, kx = a.K;
+    int rows = a.R, plane = 0;
+    if (a.stage) {
+        kx = ldx = (a.K + 63) / 64 * 64;
+        rows = plane = a.R;
+        rows *= SL;
+        const long n = (long)a.R * (kx / 8);
+        const int grid = (int)std::min((n + 255) / 256, 16L * a.num_sms);
+        const int vec = (reinterpret_cast<uintptr_t>(a.A) & 15) == 0 && (a.lda * sizeof(T)) % 16 == 0;
+        k_q4_stage<T><<<grid, 256, 0, st>>>(static_cast<const T*>(a.A), a.lda, a.R, a.K, kx,
+                                            static_cast<uint16_t*>(a.stage), vec);
+        count_launch();
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return (int)e;
+        X = a.stage;
+    }
+    const long each = a.R / std::max(1, a.offsets ? std::min(a.E, a.R) : 1);
+    if (each > 128) return launch_pair<T, 256>(a, X, ldx, rows, kx, plane, st);
+    return launch_pair<T, 128>(a, X, ldx, rows, kx, plane, st);
+}
+
+}  // namespace
+
+size_t q4_stage_bytes(const void* A, long lda, int dtype, int R, long K) {
+    if (dtype == EMU_DTYPE_F32) return (size_t)R * ((K + 63) / 64 * 64) * 6;
+    if (lda % 8 == 0 && (reinterpret_cast<uintptr_t>(A) & 15) == 0) return 0;
+    return (size_t)R * ((K + 63) / 64 * 64) * 2;
+}
+
+int launch_q4_tiles(const Q4GemmArgs& a, void* stream) {
+    cudaStream_t st = (cudaStream_t)stream;
+    if (a.dtype == EMU_DTYPE_F32) return launch_t<float>(a, st);
+    if (a.dtype == EMU_DTYPE_F16) return launch_t<__half>(a, st);
+    return launch_t<__nv_bfloat16>(a, st);
+}
+
+}  // namespace emu

@@ -41,8 +41,19 @@ emugemm_status_t q4_product(emugemm_handle_t handle, int R, int E, int N, long K
     a.packed = packed;
     a.offsets = experts ? offsets : nullptr;
     a.num_sms = h->num_sms;
+    a.err = h->err_dev;
+    const int with = experts ? (E < R ? E : R) : 1;   // experts that can have rows
+    const long cols = (long)(R / with) * (dtype == EMU_DTYPE_F32 ? 3 : 1);
+    if (cols <= 48) {
+        ProfScope ps(h, kProfQ4);
+        return from_cuda(launch_q4_rows(a, h->stream));
+    }
+    if (const size_t bytes = q4_stage_bytes(A, lda, dtype, R, K)) {
+        a.stage = ws_get_kept(h, kWsQ4X, bytes);
+        if (!a.stage) return EMUGEMM_STATUS_MEMORY_ERROR;
+    }
     ProfScope ps(h, kProfQ4);
-    return from_cuda(launch_q4_rows(a, h->stream));
+    return from_cuda(launch_q4_tiles(a, h->stream));
 }
 
 emugemm_status_t rows_checked(Handle* h, int T, int topk, int H, int dtype, long ld1, long ld2, long ld3) {
