@@ -6,10 +6,10 @@
 // cores' truncating accumulation never runs over more than 128 values of K. FP32 A is three bf16 slices (lo, mid, hi
 // multiplied in this order into the same accumulator).
 //
-// Per CTA of a pair: 128 weight rows, TN / 2 rows of A. Four converter warps turn the codes (one 16-byte load is rows g
+// Per CTA of a pair: 128 weight rows, TN / 2 rows of A. Six converter warps turn the codes (one 16-byte load is rows g
 // and g + 8 at two 8-value chunks) into the 128-byte-swizzled K-major operand in shared memory, rows of A come by TMA,
-// each CTA's part completing on the leader's barrier. Warps: warpgroup 0 = TMA producer, MMA issuer (leader) / TMEM
-// allocator; 1 = converters; 2-3 = scale, sum and store. Registers per warpgroup with setmaxnreg: 80 / 80 / 176 / 176 of
+// each CTA's part completing on the leader's barrier. Warps: 0 = TMA producer, 1 = MMA issuer (leader) and TMEM
+// allocator, 2-7 converters, warpgroups 2-3 = scale, sum and store. Registers per warpgroup with setmaxnreg: 80 / 80 / 176 / 176 of
 // the launch's 512 x 128. The peer's converters report to the leader by 16-byte bulk copies (as in k_tc_fused.cu).
 // All waits are bounded.
 #include "device_utils.cuh"
@@ -30,32 +30,30 @@ using namespace dev;
 using namespace q4;
 
 constexpr int kThreads = 512;
-constexpr int kEpiWarps = 8, kConvWarps = 4;
+constexpr int kEpiWarps = 8, kConvPairs = 3;  // converter warps 2 .. 7 in pairs, a pair per panel in turn
 constexpr int kRegEpi = 176, kRegOther = 80;
 static_assert(2 * 128 * kRegEpi + 2 * 128 * kRegOther == kThreads * 128, "register split");
-constexpr int kPanelA = 128 * 128;            // bytes of 128 weight rows x 64 values
-constexpr int kMaxStages = 6, kMaxBufs = 4;
+constexpr int kPanelA = 128 * 128;            // bytes of a panel of the weights: 128 rows x 64 values of K
+constexpr int kMaxStages = 8, kMaxBufs = 4;
 constexpr int kSmemMax = 227 * 1024;
+constexpr int kSmemFixed = 1024 + 1024 + (kMaxExperts + 1) * 4;   // alignment, barriers, row tiles of the experts
 
-// SL: slices of A's rows (1 or 3); a stage holds PP panels of 64 values of K.
+// A stage is one panel: 128 converted weight rows and TN / 2 rows of A (SL slices).
 template <int SL, int TN>
 struct Cfg {
-    static constexpr int PP = SL == 1 ? 2 : 1;
-    static constexpr int PANEL_B = TN / 2 * 128;                  // bytes of one slice, 64 values
-    static constexpr int A_BYTES = PP * kPanelA, B_BYTES = PP * SL * PANEL_B;
-    static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int FIXED = 1024 + 1024;                     // alignment, barriers
-    static constexpr int STAGES = (kSmemMax - FIXED - (kMaxExperts + 1) * 4) / STAGE < kMaxStages
-                                      ? (kSmemMax - FIXED - (kMaxExperts + 1) * 4) / STAGE : kMaxStages;
+    static constexpr int PANEL_B = TN / 2 * 128;                  // bytes of one slice
+    static constexpr int B_BYTES = SL * PANEL_B;
+    static constexpr int STAGE = kPanelA + B_BYTES;
+    static constexpr int FIT = (kSmemMax - kSmemFixed) / STAGE;
+    static constexpr int STAGES = FIT < kMaxStages ? FIT : kMaxStages;
     static constexpr int BUFS = 512 / TN < kMaxBufs ? 512 / TN : kMaxBufs;
-    static constexpr int SMEM = STAGES * STAGE + FIXED + (kMaxExperts + 1) * 4;
-    static_assert(STAGES >= 2 && SMEM <= kSmemMax, "shared memory");
-    static_assert(STAGE % 1024 == 0 && PANEL_B % 1024 == 0, "swizzle atoms");
+    static constexpr int SMEM = STAGES * STAGE + kSmemFixed;
+    static_assert(STAGES >= 3 && SMEM <= kSmemMax, "shared memory");
+    static_assert(PANEL_B % 1024 == 0, "swizzle atoms");
 };
 
 struct Ctl {
-    uint64_t b_full[kMaxStages];    // leader: the rows of A of both CTAs have landed
-    uint64_t a_full[kMaxStages];    // leader: both CTAs' weights are converted
+    uint64_t full[kMaxStages];      // leader: the rows of A of both CTAs have landed, both CTAs' weights are converted
     uint64_t empty[kMaxStages];     // both: the leader's commit
     uint64_t tmem_full[kMaxBufs];   // both: the leader's commit
     uint64_t tmem_empty[kMaxBufs];  // leader: 2 x 8 epilogue warps
@@ -63,7 +61,7 @@ struct Ctl {
     uint32_t tmem_base;
     int abort;
     alignas(16) uint32_t sig_src[4];
-    alignas(16) uint32_t sig_dst[kConvWarps][4];
+    alignas(16) uint32_t sig_dst[2 * kConvPairs][4];
 };
 static_assert(sizeof(Ctl) <= 1024, "barriers");
 
@@ -73,8 +71,7 @@ struct Params {
     const int* offsets;             // null: one matrix
     int R, E, N;
     int num_n;                      // 256-row tiles of the weights
-    int nst;                        // stages per tile
-    int group;
+    int np;                         // panels per tile (even)
     int plane;                      // rows between the slices of A (SL = 3)
     unsigned* err;
 };
@@ -93,6 +90,31 @@ template <int N>
 __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// The bounded wait of device_utils.cuh with everything but the first try out of line: the loops of the roles stay short
+// straight code (with the waits' loops inlined, fetching instructions held the MMA issuer to 280 cycles per k16 step).
+__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort, unsigned* err, unsigned bit) {
+    return mbar_wait(bar, parity, abort, err, bit);
+}
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort, unsigned* err, unsigned bit) {
+    return mbar_try_wait(smem_u32(bar), parity) || wait_slow(bar, parity, abort, err, bit);
+}
+
+// One lane of the (converged) warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
+// wait::ld that the values read depend on, so that no use of them can be moved before it.
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
 
 // The tile's expert, 256-row block of weights, and rows [m0, m1) of A. first[e] is the first row tile of expert e.
 struct Tile { int e, nb, m0, m1; };
@@ -119,13 +141,13 @@ __device__ __forceinline__ Tile tile_of(const Params& p, const int* first, int t
     return r;
 }
 
-// T: type of A and C. TN: rows of A per tile of the pair.
-template <typename T, int TN>
+// T: type of A and C. TN: rows of A per tile of the pair. GROUP: values of K per scale.
+template <typename T, int TN, int GROUP>
 __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__ CUtensorMap tm_x, Params p) {
     constexpr bool BF16 = !std::is_same<T, __half>::value;
     constexpr int SL = sizeof(T) == 4 ? 3 : 1;
     using C_ = Cfg<SL, TN>;
-    constexpr int PP = C_::PP, ST = C_::STAGES, NB = C_::BUFS;
+    constexpr int ST = C_::STAGES, NB = C_::BUFS;
     constexpr uint32_t kIdesc = idesc_f16(256, TN, BF16);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -140,8 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; ++s) {
-            mbar_init(&ctl->b_full[s], 1);
-            mbar_init(&ctl->a_full[s], kConvWarps);
+            mbar_init(&ctl->full[s], 3);       // the producer and the leader's two converter warps of the panel
             mbar_init(&ctl->empty[s], 1);
         }
         for (int b = 0; b < NB; ++b) {
@@ -184,160 +205,157 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
         reg_dec<kRegOther>();
         if (warp == 0 && lane == 0) {
             // ---------------- TMA producer: this CTA's half of the rows of A ----------------
-            const uint32_t lead_full0 = mapa_shared(smem_u32(&ctl->b_full[0]), 0);
+            const uint32_t lead_full0 = mapa_shared(smem_u32(&ctl->full[0]), 0);
             long it = 0;
             bool ok = true;
             for (int t = pair; t < num_tiles && ok; t += num_pairs) {
                 const Tile tl = tile_of<TN>(p, first, t);
                 const int row = tl.m0 + (int)rank * (TN / 2);
-                for (int kst = 0; kst < p.nst; ++kst, ++it) {
+                for (int k = 0; k < p.np; ++k, ++it) {
                     const int s = (int)(it % ST);
-                    if (!mbar_wait_cluster(&ctl->empty[s], (uint32_t)((it / ST) & 1) ^ 1u, abort, p.err,
-                                           kErrTimeoutProducer)) {
+                    if (!wait(&ctl->empty[s], (uint32_t)((it / ST) & 1) ^ 1u, abort, p.err, kErrTimeoutProducer)) {
                         ok = false;
                         break;
                     }
-                    if (leader) mbar_arrive_expect_tx(&ctl->b_full[s], 2 * C_::B_BYTES);
+                    // both CTAs' rows, and the 16-byte signals of the peer's two converter warps
+                    if (leader) mbar_arrive_expect_tx(&ctl->full[s], 2 * C_::B_BYTES + 2 * 16);
                     const uint32_t fb = lead_full0 + (uint32_t)(s * sizeof(uint64_t));
-                    uint8_t* st = smem + s * C_::STAGE + C_::A_BYTES;
+                    uint8_t* st = smem + s * C_::STAGE + kPanelA;
 #pragma unroll
-                    for (int pn = 0; pn < PP; ++pn)
-#pragma unroll
-                        for (int sl = 0; sl < SL; ++sl)
-                            tma_load_2d_pair(st + (pn * SL + sl) * C_::PANEL_B, &tm_x, fb, (kst * PP + pn) * 64,
-                                             sl * p.plane + row);
+                    for (int sl = 0; sl < SL; ++sl)
+                        tma_load_2d_pair(st + sl * C_::PANEL_B, &tm_x, fb, k * 64, sl * p.plane + row);
                 }
             }
             if (!ok) {
                 abort_pair(ctl, peer);
                 if (leader)
                     for (long j = it > ST ? it - ST : 0; j < it; ++j)
-                        drain_wait(&ctl->b_full[j % ST], (uint32_t)((j / ST) & 1));
+                        drain_wait(&ctl->full[j % ST], (uint32_t)((j / ST) & 1));
             }
-        } else if (warp == 1 && lane == 0 && leader) {
+        } else if (warp == 1 && leader) {
             // ---------------- leader: pair MMA issuer ----------------
-            const int spg = p.group / 16;          // k16 steps per scale group
-            long it = 0, ch = 0;
+            // The whole warp runs the loop and one elected lane issues: descriptors and addresses then are warp-uniform
+            // (one lane alone in a divergent loop took twice as long per panel as its four MMAs).
+            constexpr int GPP = GROUP < 64 ? 64 / GROUP : 1, PPG = GROUP > 64 ? GROUP / 64 : 1;
+            const uint64_t a00 = sdesc_kmajor(smem_u32(smem), 128);
+            int s = 0, u = 0;                      // stage and accumulator, with their phases
+            uint32_t ph = 0, pu = 1;
             bool ok = true;
             for (int t = pair; t < num_tiles && ok; t += num_pairs) {
-                int step = 0;
-                for (int kst = 0; kst < p.nst && ok; ++kst, ++it) {
-                    const int s = (int)(it % ST);
-                    const uint32_t ph = (uint32_t)((it / ST) & 1);
-                    if (!mbar_wait_cluster(&ctl->b_full[s], ph, abort, p.err, kErrTimeoutMma) ||
-                        !mbar_wait_cluster(&ctl->a_full[s], ph, abort, p.err, kErrTimeoutMma)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t sa = smem_u32(smem + s * C_::STAGE), sb = sa + C_::A_BYTES;
-                    for (int pn = 0; pn < PP && ok; ++pn) {
-                        const uint64_t a = sdesc_kmajor(sa + pn * kPanelA, 128);
-                        const uint64_t b = sdesc_kmajor(sb + pn * SL * C_::PANEL_B, 128);
-                        for (int ks = 0; ks < 4; ++ks, ++step) {
-                            const int u = (int)(ch % NB);
-                            if (step % spg == 0) {
-                                if (!mbar_wait_cluster(&ctl->tmem_empty[u], (uint32_t)((ch / NB) & 1) ^ 1u, abort, p.err,
-                                                       kErrTimeoutMma)) {
-                                    ok = false;
-                                    break;
-                                }
-                                tc_fence_after();
-                            }
-                            const uint32_t d = tmem_base + (uint32_t)(u * TN);
-                            const uint64_t adv = (uint64_t)(ks * 32) >> 4;
+                for (int k = 0; k < p.np && ok; k += PPG) {
 #pragma unroll
-                            for (int sl = SL - 1; sl >= 0; --sl)
-                                mma_f16_ss_pair(d, a + adv, b + adv + (uint64_t)((sl * C_::PANEL_B) >> 4), kIdesc,
-                                                step % spg != 0 || sl != SL - 1 ? 1u : 0u);
-                            if (step % spg == spg - 1) {
-                                mma_commit_pair_both(&ctl->tmem_full[u], (uint16_t)0x3);
-                                ++ch;
+                    for (int h = 0; h < PPG && ok; ++h) {
+                        bool ready = wait(&ctl->full[s], ph, abort, p.err, kErrTimeoutMma);
+                        const uint64_t a0 = a00 + (uint64_t)(uint32_t)((s * C_::STAGE) >> 4);
+#pragma unroll
+                        for (int q = 0; q < GPP; ++q) {
+                            if (h == 0) ready = ready && wait(&ctl->tmem_empty[u], pu, abort, p.err, kErrTimeoutMma);
+                            if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
+                            tc_fence_after();
+                            const uint32_t d = tmem_base + (uint32_t)(u * TN);
+                            if (elect_one()) {
+#pragma unroll
+                                for (int j = 0; j < 4 / GPP; ++j)
+#pragma unroll
+                                    for (int sl = SL - 1; sl >= 0; --sl) {
+                                        const uint64_t a = a0 + (uint64_t)(((q * (4 / GPP) + j) * 32) >> 4);
+                                        mma_f16_ss_pair(d, a, a + (uint64_t)((kPanelA + sl * C_::PANEL_B) >> 4), kIdesc,
+                                                        h != 0 || j != 0 || sl != SL - 1 ? 1u : 0u);
+                                    }
+                                if (h == PPG - 1) mma_commit_pair_both(&ctl->tmem_full[u], (uint16_t)0x3);
+                                if (q == GPP - 1) mma_commit_pair_both(&ctl->empty[s], (uint16_t)0x3);
                             }
+                            if (h == PPG - 1 && ++u == NB) { u = 0; pu ^= 1u; }
                         }
+                        if (++s == ST) { s = 0; ph ^= 1u; }
                     }
-                    if (!ok) break;
-                    mma_commit_pair_both(&ctl->empty[s], (uint16_t)0x3);
                 }
             }
-            if (!ok) {
+            if (!ok && elect_one()) {
                 abort_pair(ctl, peer);
                 mma_commit_pair(&ctl->drain);
                 drain_wait(&ctl->drain, 0);
             }
-        } else if (warp >= 4) {
+        } else if (warp >= 2) {
             // ---------------- converters: codes -> integers in the swizzled K-major operand ----------------
-            const int cw = warp - 4, g = lane >> 2, t4 = lane & 3;
-            const uint32_t lead_full0 = mapa_shared(smem_u32(&ctl->a_full[0]), 0);
-            const uint32_t lead_slot = mapa_shared(smem_u32(&ctl->sig_dst[cw][0]), 0);
+            // A pair of warps takes every third panel of the pair's tiles, each warp 64 of the CTA's 128 weight rows.
+            const int cp = (warp - 2) >> 1, cw = warp & 1, g = lane >> 2, t4 = lane & 3;
+            const uint32_t lead_full0 = mapa_shared(smem_u32(&ctl->full[0]), 0);
+            const uint32_t lead_slot = mapa_shared(smem_u32(&ctl->sig_dst[2 * cp + cw][0]), 0);
             const uint32_t sig_src = smem_u32(&ctl->sig_src[0]);
             const uint4 none = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
             const uint4* codes = reinterpret_cast<const uint4*>(p.packed);
             const bool odd = g & 1;
-            long it = 0;
-            bool ok = true;
-            for (int t = pair; t < num_tiles && ok; t += num_pairs) {
+            int t = pair, k = cp;                  // tile and panel to load next
+            const uint4* src = nullptr;
+            int rows = 0;                          // row blocks of 16 that this warp has in the tile
+            auto enter = [&]() {
                 const Tile tl = tile_of<TN>(p, first, t);
-                const long rb = (long)tl.nb * 16 + (long)rank * 8 + 2 * cw;   // this warp's two row blocks of 16
-                const uint4* src = codes + (((size_t)tl.e * p.l.nb + rb) * p.l.kb) * 32 + lane;
-                auto load = [&](int kst, uint4 (&c)[2][PP]) {
+                const long rb = (long)tl.nb * 16 + (long)rank * 8 + 4 * cw;
+                rows = (int)min(4L, p.l.nb - rb);
+                src = codes + (((size_t)tl.e * p.l.nb + rb) * p.l.kb) * 32 + lane;
+            };
+            auto load = [&](uint4 (&c)[4]) {
 #pragma unroll
-                    for (int r = 0; r < 2; ++r)
+                for (int r = 0; r < 4; ++r)
+                    c[r] = r < rows && k < p.l.kb ? __ldg(src + ((size_t)r * p.l.kb + k) * 32) : none;
+            };
+            auto settle = [&]() {                  // the panel's tile, when k has run past the end of one
+                bool moved = false;
+                while (k >= p.np && t < num_tiles) {
+                    k -= p.np;
+                    t += num_pairs;
+                    moved = true;
+                }
+                if (moved && t < num_tiles) enter();
+            };
+            uint4 next[4] = {none, none, none, none};
+            if (t < num_tiles) {
+                enter();
+                settle();
+                if (t < num_tiles) load(next);
+            }
+            for (long it = cp; t < num_tiles; it += kConvPairs) {
+                const int s = (int)(it % ST);
+                uint4 c[4];
 #pragma unroll
-                        for (int pn = 0; pn < PP; ++pn) {
-                            const long kb = (long)kst * PP + pn;
-                            c[r][pn] = rb + r < p.l.nb && kb < p.l.kb ? __ldg(src + ((size_t)r * p.l.kb + kb) * 32) : none;
-                        }
-                };
-                uint4 next[2][PP];
-                load(0, next);
-                for (int kst = 0; kst < p.nst; ++kst, ++it) {
-                    const int s = (int)(it % ST);
-                    uint4 c[2][PP];
+                for (int r = 0; r < 4; ++r) c[r] = next[r];
+                k += kConvPairs;
+                settle();
+                const bool more = t < num_tiles;
+                if (more) load(next);
+                const bool ready = wait(&ctl->empty[s], (uint32_t)((it / ST) & 1) ^ 1u, abort, p.err, kErrTimeoutConvert);
+                if (!__all_sync(0xffffffffu, ready)) {
+                    if (lane == 0) abort_pair(ctl, peer);
+                    break;
+                }
+                uint8_t* st = smem + s * C_::STAGE + cw * 64 * 128;
 #pragma unroll
-                    for (int r = 0; r < 2; ++r)
+                for (int r = 0; r < 4; ++r) {
+                    // rows g and g + 8, chunks t4 and 4 + t4; odd rows store the upper chunk first, so that the eight
+                    // lanes of a store phase (two rows) touch all eight 16-byte columns
 #pragma unroll
-                        for (int pn = 0; pn < PP; ++pn) c[r][pn] = next[r][pn];
-                    if (kst + 1 < p.nst) load(kst + 1, next);
-                    const bool ready = mbar_wait_cluster(&ctl->empty[s], (uint32_t)((it / ST) & 1) ^ 1u, abort, p.err,
-                                                         kErrTimeoutConvert);
-                    if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
-                    uint8_t* st = smem + s * C_::STAGE;
-#pragma unroll
-                    for (int pn = 0; pn < PP; ++pn)
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            // rows g and g + 8, chunks t4 and 4 + t4; odd rows store the upper chunk first, so that the
-                            // eight lanes of a store phase (two rows) touch all eight 16-byte columns
-#pragma unroll
-                            for (int half = 0; half < 2; ++half) {
-                                const int row = (2 * cw + r) * 16 + g + 8 * half;
-                                const uint32_t lo = half ? c[r][pn].y : c[r][pn].x, hi = half ? c[r][pn].w : c[r][pn].z;
-                                const uint32_t w0 = odd ? hi : lo, w1 = odd ? lo : hi;
-                                const int c0 = odd ? 4 + t4 : t4, c1 = c0 ^ 4;
-                                uint8_t* o = st + pn * kPanelA + row * 128;
-                                uint4 v;
-                                v.x = code_pair<BF16>(w0, 0); v.y = code_pair<BF16>(w0, 1);
-                                v.z = code_pair<BF16>(w0, 2); v.w = code_pair<BF16>(w0, 3);
-                                *reinterpret_cast<uint4*>(o + ((c0 ^ g) << 4)) = v;
-                                v.x = code_pair<BF16>(w1, 0); v.y = code_pair<BF16>(w1, 1);
-                                v.z = code_pair<BF16>(w1, 2); v.w = code_pair<BF16>(w1, 3);
-                                *reinterpret_cast<uint4*>(o + ((c1 ^ g) << 4)) = v;
-                            }
-                        }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (leader) {
-                            if (cw == 0) mbar_arrive_expect_tx(&ctl->a_full[s], 16 * kConvWarps);
-                            else mbar_arrive(&ctl->a_full[s]);
-                        } else {
-                            bulk_signal_cluster(lead_slot, sig_src, 16, lead_full0 + (uint32_t)(s * sizeof(uint64_t)));
-                        }
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t lo = half ? c[r].y : c[r].x, hi = half ? c[r].w : c[r].z;
+                        const uint32_t w0 = odd ? hi : lo, w1 = odd ? lo : hi;
+                        const int c0 = odd ? 4 + t4 : t4, c1 = c0 ^ 4;
+                        uint8_t* o = st + (r * 16 + g + 8 * half) * 128;
+                        uint4 v;
+                        v.x = code_pair<BF16>(w0, 0); v.y = code_pair<BF16>(w0, 1);
+                        v.z = code_pair<BF16>(w0, 2); v.w = code_pair<BF16>(w0, 3);
+                        *reinterpret_cast<uint4*>(o + ((c0 ^ g) << 4)) = v;
+                        v.x = code_pair<BF16>(w1, 0); v.y = code_pair<BF16>(w1, 1);
+                        v.z = code_pair<BF16>(w1, 2); v.w = code_pair<BF16>(w1, 3);
+                        *reinterpret_cast<uint4*>(o + ((c1 ^ g) << 4)) = v;
                     }
                 }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    if (leader) mbar_arrive(&ctl->full[s]);
+                    else bulk_signal_cluster(lead_slot, sig_src, 16, lead_full0 + (uint32_t)(s * sizeof(uint64_t)));
+                }
             }
-            if (!ok && lane == 0) abort_pair(ctl, peer);
         }
     } else {
         reg_inc<kRegEpi>();
@@ -347,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
         const uint32_t lane_off = (uint32_t)(sp * 32) << 16;
         const uint32_t lead_te0 = mapa_shared(smem_u32(&ctl->tmem_empty[0]), 0);
         const uint16_t* scales = reinterpret_cast<const uint16_t*>(p.packed + p.l.scales_at);
-        const int groups = p.nst * PP * 64 / p.group;      // of the padded K
+        const int groups = p.np * 64 / GROUP;              // of the padded K
         constexpr int H = TN / 2;
         long ch = 0;
         bool ok = true;
@@ -364,18 +382,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
                 const int u = (int)(ch % NB);
                 const float s = s_next;
                 s_next = there && gi + 1 < p.l.groups ? __uint_as_float((uint32_t)__ldg(sc + (gi + 1) * 16) << 16) : 0.f;
-                const bool ready = mbar_wait_cluster(&ctl->tmem_full[u], (uint32_t)((ch / NB) & 1), abort, p.err,
-                                                     kErrTimeoutEpilogue);
+                const bool ready = mbar_wait(&ctl->tmem_full[u], (uint32_t)((ch / NB) & 1), abort, p.err,
+                                             kErrTimeoutEpilogue);   // inline: a call would save the sums around it
                 if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t tb = tmem_base + lane_off + (uint32_t)(u * TN + half * H);
+                uint32_t r[2][16];                 // a read runs while the previous one is added
+                tmem_ld_32x32b_x16(tb, r[0]);
 #pragma unroll
                 for (int q = 0; q < H / 16; ++q) {
-                    uint32_t r[16];
-                    tmem_ld_32x32b_x16(tb + (uint32_t)(q * 16), r);
-                    tmem_ld_wait();
+                    tmem_ld_wait_for(r[q & 1]);
+                    if (q + 1 < H / 16) tmem_ld_32x32b_x16(tb + (uint32_t)((q + 1) * 16), r[(q + 1) & 1]);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) sum[q * 16 + j] = fmaf(s, __uint_as_float(r[j]), sum[q * 16 + j]);
+                    for (int j = 0; j < 16; ++j)
+                        sum[q * 16 + j] = fmaf(s, __uint_as_float(r[q & 1][j]), sum[q * 16 + j]);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -431,8 +451,8 @@ __global__ void __launch_bounds__(256) k_q4_stage(const T* __restrict__ A, long 
     }
 }
 
-template <typename T, int TN>
-int launch_pair(const Q4GemmArgs& a, const void* X, long ldx, int rows, long kx, int plane, cudaStream_t st) {
+template <typename T, int TN, int GROUP>
+int launch_pair_g(const Q4GemmArgs& a, const void* X, long ldx, int rows, long kx, int plane, cudaStream_t st) {
     constexpr int SL = sizeof(T) == 4 ? 3 : 1;
     using C_ = Cfg<SL, TN>;
     PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
@@ -453,11 +473,10 @@ int launch_pair(const Q4GemmArgs& a, const void* X, long ldx, int rows, long kx,
     p.offsets = a.offsets;
     p.R = a.R; p.E = a.E; p.N = a.N;
     p.num_n = (a.N + 255) / 256;
-    p.nst = (int)((a.K + 127) / 128 * (2 / C_::PP));
-    p.group = a.group;
+    p.np = (int)((a.K + 127) / 128 * 2);
     p.plane = plane;
     p.err = a.err;
-    auto kern = k_q4_pair<T, TN>;
+    auto kern = k_q4_pair<T, TN, GROUP>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM);
     if (e != cudaSuccess) return (int)e;
     // with offsets the number of tiles is known on the device only: at most one partly filled tile per expert
@@ -478,6 +497,13 @@ int launch_pair(const Q4GemmArgs& a, const void* X, long ldx, int rows, long kx,
     count_launch();
     if (e != cudaSuccess) return (int)e;
     return (int)cudaGetLastError();
+}
+
+template <typename T, int TN>
+int launch_pair(const Q4GemmArgs& a, const void* X, long ldx, int rows, long kx, int plane, cudaStream_t st) {
+    if (a.group == 32) return launch_pair_g<T, TN, 32>(a, X, ldx, rows, kx, plane, st);
+    if (a.group == 64) return launch_pair_g<T, TN, 64>(a, X, ldx, rows, kx, plane, st);
+    return launch_pair_g<T, TN, 128>(a, X, ldx, rows, kx, plane, st);
 }
 
 template <typename T>
