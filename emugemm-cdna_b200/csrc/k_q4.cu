@@ -158,11 +158,14 @@ __global__ void __launch_bounds__(256) k_q4_unpack(const uint8_t* __restrict__ p
 // One warp multiplies row blocks of 16 weights rows with up to 8 NT columns by m16n8k16 products: the weights are the
 // 16-row operand (their integers are exact in bf16 and fp16), the columns are rows of A, and for FP32 A the three bf16
 // slices of each row (exact to 24 bits). A group's sum is kept apart and added to the row's FP32 sum times its scale,
-// so no weight is ever rounded. What bounds it is the read of the codes. The columns of the block's K range lie in
-// shared memory (rows 64 bytes apart modulo 128, so that the 16-byte fragment loads of 8 rows x 4 lanes meet no
-// bank conflict); each warp of a row block takes every WK-th 128 values of K, the partial sums are added in order, and
-// where there are few row blocks a cluster of CTAs splits K and adds its parts over distributed shared memory.
+// so no weight is ever rounded. What bounds it is the read of the codes (and, beyond about 16 columns, the products):
+// each warp keeps the codes of its next D x 128 values of K in flight in registers, the first of them from before the
+// columns are staged. The columns of the block's K range lie in shared memory (rows 64 bytes apart modulo 128, so that
+// the 16-byte fragment loads of 8 rows x 4 lanes meet no bank conflict); the WK warps of a row block take 128 values
+// of K in turn, their sums are added in order, and where there are few row blocks a cluster of CTAs splits K and adds
+// its parts over distributed shared memory.
 constexpr int kWarps = 8;
+constexpr int kRowsSmem = 100 * 1024; // two CTAs on an SM
 
 struct RowsParams {
     const void* A; long lda;
@@ -172,6 +175,7 @@ struct RowsParams {
     int R, E, N; long K;
     int kspan;                // K values per CTA of the cluster (a multiple of 128)
     int kstage;               // K values staged at a time (a multiple of 128)
+    int vec;                  // rows of A on 16-byte boundaries
 };
 
 template <bool BF16>
@@ -241,9 +245,14 @@ __device__ __forceinline__ bool nth_expert(const int* offsets, int E, int i, int
     return false;
 }
 
-// T: type of A and C; NT: column tiles of 8; WR: warps over row blocks; RBW: row blocks per warp; GROUP.
-template <typename T, int NT, int WR, int RBW, int GROUP>
-__global__ void __launch_bounds__(32 * kWarps) k_q4_rows(RowsParams p) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {   // the rest of 16 is zeroed
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// T: type of A and C; NT: column tiles of 8; WR: warps over row blocks; RBW: row blocks per warp; D: units of 128
+// values of K in flight per warp; GROUP.
+template <typename T, int NT, int WR, int RBW, int D, int GROUP>
+__global__ void __launch_bounds__(32 * kWarps, 2) k_q4_rows(RowsParams p) {
     constexpr bool BF16 = !std::is_same<T, __half>::value;
     constexpr int SL = sizeof(T) == 4 ? 3 : 1;
     constexpr int WK = kWarps / WR;
@@ -254,7 +263,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_q4_rows(RowsParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int pitch = p.kstage + 32;             // 16-bit values between columns
     uint16_t* xs = reinterpret_cast<uint16_t*>(smem);
-    float* red = reinterpret_cast<float*>(smem); // reused after the last product: [WK][ROWS][COLS]
+    float* red = reinterpret_cast<float*>(smem); // reused after the last product: [WK][COLS][ROWS]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int wr = warp % WR, wk = warp / WR;
@@ -263,9 +272,32 @@ __global__ void __launch_bounds__(32 * kWarps) k_q4_rows(RowsParams p) {
     if (p.offsets && !nth_expert(p.offsets, p.E, blockIdx.y, p.R, e, r0, r1)) return;   // the whole cluster returns
     const long rb0 = (long)(blockIdx.x / csize) * (WR * RBW);
     const long kbeg = (long)rank * p.kspan, kend = min(p.K, kbeg + p.kspan);
+    const int units = (int)((kend - kbeg + 127) / 128);          // of the CTA; this warp's are wk, wk + WK, ...
     const T* A = static_cast<const T*>(p.A);
-    const uint4* codes = reinterpret_cast<const uint4*>(p.packed);
-    const uint32_t* scales = reinterpret_cast<const uint32_t*>(p.packed + p.l.scales_at);
+    // the lane's codes and scale words of this warp's first row block, at the CTA's first value of K
+    const long rb = rb0 + wr * RBW;
+    const size_t b = (size_t)e * p.l.nb + rb;
+    const uint4* codes = reinterpret_cast<const uint4*>(p.packed) + (b * p.l.kb + kbeg / 64) * 32 + lane;
+    const uint32_t* scales = reinterpret_cast<const uint32_t*>(p.packed + p.l.scales_at) + (b * p.l.groups + kbeg / GROUP) * 8 + g;
+    const int kbs = (int)(p.l.kb - kbeg / 64), grs = (int)(p.l.groups - kbeg / GROUP);
+    const int there = (int)max(0L, min((long)RBW, p.l.nb - rb));
+
+    uint4 cd[D][RBW][2];
+    uint32_t sc[D][RBW][4 / FLUSH];
+    auto load = [&](int d, int unit) {
+#pragma unroll
+        for (int r = 0; r < RBW; ++r) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (r < there && 2 * unit + h < kbs) cd[d][r][h] = ld_codes(codes + ((size_t)r * p.l.kb + 2 * unit + h) * 32);
+                else cd[d][r][h] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+#pragma unroll
+            for (int j = 0; j < 4 / FLUSH; ++j) {
+                const int kg = unit * (128 / GROUP) + j;
+                sc[d][r][j] = r < there && kg < grs ? __ldg(scales + ((size_t)r * p.l.groups + kg) * 8) : 0u;
+            }
+        }
+    };
 
     for (int c0 = r0; c0 < r1; c0 += TOK) {
         const int toks = min(TOK, r1 - c0), cols = toks * SL;
@@ -276,90 +308,103 @@ __global__ void __launch_bounds__(32 * kWarps) k_q4_rows(RowsParams p) {
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[r][n][j] = 0.f;
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+            if (wk + d * WK < units) load(d, wk + d * WK);
 
-        for (long ks = kbeg; ks < kend; ks += p.kstage) {
-            const int len = (int)min((long)p.kstage, kend - ks);
-            const int span = (len + 127) / 128 * 128;
-            __syncthreads();
-            for (int i = threadIdx.x; i < toks * span; i += 32 * kWarps) {
-                const int m = i / span, k = i - m * span;
-                const T v = k < len ? A[(size_t)(c0 + m) * p.lda + ks + k] : from_float<T>(0.f);
-                if (SL == 3) {
-                    uint16_t s0, s1, s2;
-                    slice3(to_float<T>(v), s0, s1, s2);
-                    xs[(3 * m) * pitch + k] = s0;
-                    xs[(3 * m + 1) * pitch + k] = s1;
-                    xs[(3 * m + 2) * pitch + k] = s2;
-                } else {
-                    xs[m * pitch + k] = *reinterpret_cast<const uint16_t*>(&v);
+        int unit = wk;
+        for (int u0 = 0; u0 < units; u0 += p.kstage / 128) {     // a multiple of WK * D units, or all of them
+            const int u1 = min(units, u0 + p.kstage / 128);
+            const int span = (u1 - u0) * 128;
+            const long ks = kbeg + (long)u0 * 128;
+            if (u0) __syncthreads();
+            for (int m = 0; m < toks; ++m) {
+                const T* row = A + (size_t)(c0 + m) * p.lda + ks;
+                const int len = (int)min((long)span, p.K - ks);
+                for (int k = threadIdx.x * 8; k < span; k += 256 * kWarps) {
+                    if (SL == 1 && p.vec) {
+                        const int left = len - k;
+                        cp_async16(static_cast<uint32_t>(__cvta_generic_to_shared(xs + m * pitch + k)),
+                                   left > 0 ? row + k : A, left <= 0 ? 0 : left >= 8 ? 16 : 2 * left);
+                        continue;
+                    }
+                    T x[8];
+                    if (p.vec && k + 8 <= len) {
+#pragma unroll
+                        for (int j = 0; j < 8 * (int)sizeof(T) / 16; ++j)
+                            reinterpret_cast<uint4*>(x)[j] = __ldg(reinterpret_cast<const uint4*>(row + k) + j);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) x[j] = k + j < len ? row[k + j] : from_float<T>(0.f);
+                    }
+                    if (SL == 3) {
+                        __align__(16) uint16_t s[3][8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) slice3(to_float<T>(x[j]), s[0][j], s[1][j], s[2][j]);
+#pragma unroll
+                        for (int q = 0; q < 3; ++q)
+                            *reinterpret_cast<uint4*>(xs + (3 * m + q) * pitch + k) = *reinterpret_cast<const uint4*>(s[q]);
+                    } else {
+                        *reinterpret_cast<uint4*>(xs + m * pitch + k) = *reinterpret_cast<const uint4*>(x);
+                    }
                 }
             }
+            if (SL == 1) asm volatile("cp.async.wait_all;" ::: "memory");
             __syncthreads();
-            for (int ku = wk * 128; ku < span; ku += WK * 128) {
-                const long kb = (ks + ku) / 64;
-                uint4 cd[RBW][2];
-                uint32_t sc[RBW][4 / FLUSH];
+            const uint16_t* xk = xs + g * pitch + 8 * t - u0 * 128;
+            while (unit < u1) {
 #pragma unroll
-                for (int r = 0; r < RBW; ++r) {
-                    const long rb = rb0 + wr * RBW + r;
-                    const bool there = rb < p.l.nb;
-                    const size_t b = (size_t)e * p.l.nb + rb;
+                for (int d = 0; d < D; ++d) {
+                    if (unit >= u1) break;
+                    float tmp[RBW][NT][4];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        cd[r][h] = there && kb + h < p.l.kb ? ld_codes(codes + (b * p.l.kb + kb + h) * 32 + lane)
-                                                            : make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+                    for (int i = 0; i < 4; ++i) {   // 32 values of K: half i & 1 of tile i >> 1
+                        if (i % FLUSH == 0)
 #pragma unroll
-                    for (int j = 0; j < 4 / FLUSH; ++j) {
-                        const long kg = (ks + ku) / GROUP + j;
-                        sc[r][j] = there && kg < p.l.groups ? scales[(b * p.l.groups + kg) * 8 + g] : 0u;
-                    }
-                }
-                float tmp[RBW][NT][4];
+                            for (int r = 0; r < RBW; ++r)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {   // 32 values of K: half i & 1 of tile i >> 1
-                    if (i % FLUSH == 0)
+                                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int r = 0; r < RBW; ++r)
-#pragma unroll
-                            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) tmp[r][n][j] = 0.f;
-                    uint32_t a[RBW][2][4];
-#pragma unroll
-                    for (int r = 0; r < RBW; ++r) {
-                        const uint4 c = cd[r][i >> 1];
-                        const uint32_t w0 = (i & 1) ? c.z : c.x, w1 = (i & 1) ? c.w : c.y;
-#pragma unroll
-                        for (int s = 0; s < 2; ++s) {
-                            a[r][s][0] = code_pair<BF16>(w0, 2 * s);
-                            a[r][s][1] = code_pair<BF16>(w1, 2 * s);
-                            a[r][s][2] = code_pair<BF16>(w0, 2 * s + 1);
-                            a[r][s][3] = code_pair<BF16>(w1, 2 * s + 1);
-                        }
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        uint4 x = make_uint4(0, 0, 0, 0);
-                        if (8 * n + g < cols)
-                            x = *reinterpret_cast<const uint4*>(xs + (8 * n + g) * pitch + ku + 32 * i + 8 * t);
+                                    for (int j = 0; j < 4; ++j) tmp[r][n][j] = 0.f;
+                        uint32_t a[RBW][2][4];
 #pragma unroll
                         for (int r = 0; r < RBW; ++r) {
-                            mma16816<BF16>(tmp[r][n], a[r][0][0], a[r][0][1], a[r][0][2], a[r][0][3], x.x, x.y);
-                            mma16816<BF16>(tmp[r][n], a[r][1][0], a[r][1][1], a[r][1][2], a[r][1][3], x.z, x.w);
-                        }
-                    }
-                    if (i % FLUSH == FLUSH - 1)
+                            const uint4 c = cd[d][r][i >> 1];
+                            const uint32_t w0 = (i & 1) ? c.z : c.x, w1 = (i & 1) ? c.w : c.y;
 #pragma unroll
-                        for (int r = 0; r < RBW; ++r) {
-                            const float s0 = bf16_lo(sc[r][i / FLUSH]), s1 = bf16_hi(sc[r][i / FLUSH]);
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) {
-                                acc[r][n][0] = fmaf(s0, tmp[r][n][0], acc[r][n][0]);
-                                acc[r][n][1] = fmaf(s0, tmp[r][n][1], acc[r][n][1]);
-                                acc[r][n][2] = fmaf(s1, tmp[r][n][2], acc[r][n][2]);
-                                acc[r][n][3] = fmaf(s1, tmp[r][n][3], acc[r][n][3]);
+                            for (int s = 0; s < 2; ++s) {
+                                a[r][s][0] = code_pair<BF16>(w0, 2 * s);
+                                a[r][s][1] = code_pair<BF16>(w1, 2 * s);
+                                a[r][s][2] = code_pair<BF16>(w0, 2 * s + 1);
+                                a[r][s][3] = code_pair<BF16>(w1, 2 * s + 1);
                             }
                         }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            uint4 x = make_uint4(0, 0, 0, 0);
+                            if (8 * n + g < cols)
+                                x = *reinterpret_cast<const uint4*>(xk + 8 * n * pitch + unit * 128 + 32 * i);
+#pragma unroll
+                            for (int r = 0; r < RBW; ++r) {
+                                mma16816<BF16>(tmp[r][n], a[r][0][0], a[r][0][1], a[r][0][2], a[r][0][3], x.x, x.y);
+                                mma16816<BF16>(tmp[r][n], a[r][1][0], a[r][1][1], a[r][1][2], a[r][1][3], x.z, x.w);
+                            }
+                        }
+                        if (i % FLUSH == FLUSH - 1)
+#pragma unroll
+                            for (int r = 0; r < RBW; ++r) {
+                                const float s0 = bf16_lo(sc[d][r][i / FLUSH]), s1 = bf16_hi(sc[d][r][i / FLUSH]);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    acc[r][n][0] = fmaf(s0, tmp[r][n][0], acc[r][n][0]);
+                                    acc[r][n][1] = fmaf(s0, tmp[r][n][1], acc[r][n][1]);
+                                    acc[r][n][2] = fmaf(s1, tmp[r][n][2], acc[r][n][2]);
+                                    acc[r][n][3] = fmaf(s1, tmp[r][n][3], acc[r][n][3]);
+                                }
+                            }
+                    }
+                    if (unit + D * WK < units) load(d, unit + D * WK);
+                    unit += WK;
                 }
             }
         }
@@ -390,28 +435,34 @@ __global__ void __launch_bounds__(32 * kWarps) k_q4_rows(RowsParams p) {
                     }
             if (n < p.N) static_cast<T*>(p.C)[(size_t)(c0 + m) * p.ldc + n] = from_float<T>(y);
         }
-        if (csize > 1) cluster_sync();   // the next pass, or the exit, waits for the others' reads
+        // the next pass, or the exit, waits for the others' reads
+        if (csize > 1) cluster_sync();
+        else __syncthreads();
     }
 }
 
-template <typename T, int NT, int WR, int RBW, int GROUP>
+template <typename T, int NT, int WR, int RBW, int D, int GROUP>
 int launch_rows_g(RowsParams p, int num_sms, cudaStream_t st) {
     constexpr int SL = sizeof(T) == 4 ? 3 : 1;
+    constexpr int STEP = kWarps / WR * D * 128;                // values of K that the warps hold in flight
     const long groups = (p.l.nb + WR * RBW - 1) / (WR * RBW);
     const int experts = p.offsets ? std::min(p.E, p.R) : 1;
-    // K split over a cluster while the CTAs do not fill the GPU twice and each keeps at least 512 values of K
+    // K split over a cluster while the CTAs do not fill the GPU twice and each keeps a step of the warps
     int ck = 1;
-    while (ck < 8 && groups * experts * ck < 2L * num_sms && p.K >= 512L * 2 * ck) ck *= 2;
+    while (ck < 8 && groups * experts * ck < 2L * num_sms && p.K >= 2L * ck * STEP) ck *= 2;
     p.kspan = (int)(((p.K + ck - 1) / ck + 127) / 128 * 128);
     ck = (int)((p.K + p.kspan - 1) / p.kspan);
-    const int cols = std::min(8 * NT, SL * std::min(p.R, 8 * NT / SL));
-    const int most = (96 * 1024 / (2 * cols) - 32) / 128 * 128;
+    const int cols = SL * std::min(p.R, 8 * NT / SL);
+    const int most = std::max(STEP, (96 * 1024 / (2 * cols) - 32) / STEP * STEP);
     p.kstage = std::min(p.kspan, most);
+    p.vec = (reinterpret_cast<uintptr_t>(p.A) & 15) == 0 && (p.lda * sizeof(T)) % 16 == 0;
     const size_t smem = std::max((size_t)cols * (p.kstage + 32) * 2,
                                  (size_t)(kWarps / WR) * WR * RBW * 16 * 8 * NT * 4);
-    auto kern = k_q4_rows<T, NT, WR, RBW, GROUP>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
+    auto kern = k_q4_rows<T, NT, WR, RBW, D, GROUP>;
+    static OncePerDevice once;
+    const int e0 = once([&] { return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem); });
+    if (e0) return e0;
+    if (smem > (size_t)kRowsSmem) return (int)cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -423,19 +474,19 @@ int launch_rows_g(RowsParams p, int num_sms, cudaStream_t st) {
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kern, p);
+    cfg.numAttrs = ck > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
     count_launch();
     if (e != cudaSuccess) return (int)e;
     return (int)cudaGetLastError();
 }
 
-template <typename T, int NT, int WR, int RBW>
+template <typename T, int NT, int WR, int RBW, int D>
 int launch_rows_n(const RowsParams& p, int group, int num_sms, cudaStream_t st) {
     switch (group) {
-        case 32: return launch_rows_g<T, NT, WR, RBW, 32>(p, num_sms, st);
-        case 64: return launch_rows_g<T, NT, WR, RBW, 64>(p, num_sms, st);
-        default: return launch_rows_g<T, NT, WR, RBW, 128>(p, num_sms, st);
+        case 32: return launch_rows_g<T, NT, WR, RBW, D, 32>(p, num_sms, st);
+        case 64: return launch_rows_g<T, NT, WR, RBW, D, 64>(p, num_sms, st);
+        default: return launch_rows_g<T, NT, WR, RBW, D, 128>(p, num_sms, st);
     }
 }
 
@@ -443,10 +494,12 @@ template <typename T>
 int launch_rows_t(const RowsParams& p, int group, int num_sms, cudaStream_t st) {
     const int experts = p.offsets ? std::min(p.E, p.R) : 1;
     const long cols = (long)((p.R + experts - 1) / experts) * (sizeof(T) == 4 ? 3 : 1);
-    if (cols <= 8) return launch_rows_n<T, 1, 2, 1>(p, group, num_sms, st);
-    if (cols <= 16) return launch_rows_n<T, 2, 4, 1>(p, group, num_sms, st);
-    if (cols <= 24) return launch_rows_n<T, 3, 4, 2>(p, group, num_sms, st);
-    return launch_rows_n<T, 6, 4, 2>(p, group, num_sms, st);
+    if (cols <= 3) return launch_rows_n<T, 1, 1, 1, 4>(p, group, num_sms, st);
+    if (cols <= 8) return launch_rows_n<T, 1, 4, 1, 4>(p, group, num_sms, st);
+    if (cols <= 16) return launch_rows_n<T, 2, 4, 1, 4>(p, group, num_sms, st);
+    if (cols <= 24) return launch_rows_n<T, 3, 4, 2, 1>(p, group, num_sms, st);
+    if (cols <= 32) return launch_rows_n<T, 4, 4, 1, 2>(p, group, num_sms, st);
+    return launch_rows_n<T, 6, 4, 1, 2>(p, group, num_sms, st);
 }
 
 }  // namespace

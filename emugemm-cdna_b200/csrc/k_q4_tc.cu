@@ -477,8 +477,9 @@ int launch_pair_g(const Q4GemmArgs& a, const void* X, long ldx, int rows, long k
     p.plane = plane;
     p.err = a.err;
     auto kern = k_q4_pair<T, TN, GROUP>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM);
-    if (e != cudaSuccess) return (int)e;
+    static OncePerDevice once;
+    const int e0 = once([&] { return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM); });
+    if (e0) return e0;
     // with offsets the number of tiles is known on the device only: at most one partly filled tile per expert
     const long tiles = ((a.offsets ? std::min(a.E, a.R) : 0) + ((long)a.R + TN - 1) / TN) * p.num_n;
     cudaLaunchConfig_t cfg = {};
@@ -493,7 +494,7 @@ int launch_pair_g(const Q4GemmArgs& a, const void* X, long ldx, int rows, long k
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kern, tm, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tm, p);
     count_launch();
     if (e != cudaSuccess) return (int)e;
     return (int)cudaGetLastError();

@@ -12,12 +12,31 @@
 
 #include "emugemm_internal.h"
 
+#include <atomic>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 namespace emu {
+
+// Runs its argument (a cudaFuncSetAttribute call, a cudaError_t as int) until it has succeeded once on the current
+// device. Calls from several threads may run it more than once.
+struct OncePerDevice {
+    std::atomic<unsigned long long> done{0};
+    template <typename F>
+    int operator()(F&& f) {
+        int dev = 0;
+        const cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return (int)e;
+        const unsigned long long bit = 1ull << (dev & 63);
+        if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return 0;
+        const int r = f();
+        if (!r && dev < 64) done.fetch_or(bit, std::memory_order_release);
+        return r;
+    }
+};
+
 namespace q4 {
 
 struct Layout {
