@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(256) k_q4_unpack(const uint8_t* __restrict__ p
 // of K in turn, their sums are added in order, and where there are few row blocks a cluster of CTAs splits K and adds
 // its parts over distributed shared memory.
 constexpr int kWarps = 8;
-constexpr int kRowsSmem = 100 * 1024; // two CTAs on an SM
+constexpr int kRowsSmem = 100 * 1024;
 
 struct RowsParams {
     const void* A; long lda;
@@ -250,9 +250,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int by
 }
 
 // T: type of A and C; NT: column tiles of 8; WR: warps over row blocks; RBW: row blocks per warp; D: units of 128
-// values of K in flight per warp; GROUP.
-template <typename T, int NT, int WR, int RBW, int D, int GROUP>
-__global__ void __launch_bounds__(32 * kWarps, 2) k_q4_rows(RowsParams p) {
+// values of K in flight per warp; CTAS: resident on an SM; GROUP.
+template <typename T, int NT, int WR, int RBW, int D, int CTAS, int GROUP>
+__global__ void __launch_bounds__(32 * kWarps, CTAS) k_q4_rows(RowsParams p) {
     constexpr bool BF16 = !std::is_same<T, __half>::value;
     constexpr int SL = sizeof(T) == 4 ? 3 : 1;
     constexpr int WK = kWarps / WR;
@@ -274,28 +274,29 @@ __global__ void __launch_bounds__(32 * kWarps, 2) k_q4_rows(RowsParams p) {
     const long kbeg = (long)rank * p.kspan, kend = min(p.K, kbeg + p.kspan);
     const int units = (int)((kend - kbeg + 127) / 128);          // of the CTA; this warp's are wk, wk + WK, ...
     const T* A = static_cast<const T*>(p.A);
-    // the lane's codes and scale words of this warp's first row block, at the CTA's first value of K
-    const long rb = rb0 + wr * RBW;
-    const size_t b = (size_t)e * p.l.nb + rb;
-    const uint4* codes = reinterpret_cast<const uint4*>(p.packed) + (b * p.l.kb + kbeg / 64) * 32 + lane;
-    const uint32_t* scales = reinterpret_cast<const uint32_t*>(p.packed + p.l.scales_at) + (b * p.l.groups + kbeg / GROUP) * 8 + g;
-    const int kbs = (int)(p.l.kb - kbeg / 64), grs = (int)(p.l.groups - kbeg / GROUP);
-    const int there = (int)max(0L, min((long)RBW, p.l.nb - rb));
+    // The lane's codes and scale words of this warp's row blocks, at the CTA's first value of K. What lies behind the
+    // last row block, tile or group is not guarded against but read again from the last one: its products belong to
+    // rows that are not stored or meet the zeros staged behind K.
+    const uint4* codes[RBW];
+    const uint32_t* scales[RBW];
+#pragma unroll
+    for (int r = 0; r < RBW; ++r) {
+        const size_t b = (size_t)e * p.l.nb + min(rb0 + wr * RBW + r, p.l.nb - 1);
+        codes[r] = reinterpret_cast<const uint4*>(p.packed) + (b * p.l.kb + kbeg / 64) * 32 + lane;
+        scales[r] = reinterpret_cast<const uint32_t*>(p.packed + p.l.scales_at) + (b * p.l.groups + kbeg / GROUP) * 8 + g;
+    }
+    const int kb1 = (int)(p.l.kb - kbeg / 64) - 1, gr1 = (int)(p.l.groups - kbeg / GROUP) - 1;
 
     uint4 cd[D][RBW][2];
     uint32_t sc[D][RBW][4 / FLUSH];
     auto load = [&](int d, int unit) {
 #pragma unroll
         for (int r = 0; r < RBW; ++r) {
+            cd[d][r][0] = ld_codes(codes[r] + 64 * unit);
+            cd[d][r][1] = ld_codes(codes[r] + 32 * min(2 * unit + 1, kb1));
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (r < there && 2 * unit + h < kbs) cd[d][r][h] = ld_codes(codes + ((size_t)r * p.l.kb + 2 * unit + h) * 32);
-                else cd[d][r][h] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-#pragma unroll
-            for (int j = 0; j < 4 / FLUSH; ++j) {
-                const int kg = unit * (128 / GROUP) + j;
-                sc[d][r][j] = r < there && kg < grs ? __ldg(scales + ((size_t)r * p.l.groups + kg) * 8) : 0u;
-            }
+            for (int j = 0; j < 4 / FLUSH; ++j)
+                sc[d][r][j] = __ldg(scales[r] + 8 * (j ? min(unit * (4 / FLUSH) + j, gr1) : unit * (4 / FLUSH)));
         }
     };
 
@@ -351,7 +352,10 @@ __global__ void __launch_bounds__(32 * kWarps, 2) k_q4_rows(RowsParams p) {
             }
             if (SL == 1) asm volatile("cp.async.wait_all;" ::: "memory");
             __syncthreads();
-            const uint16_t* xk = xs + g * pitch + 8 * t - u0 * 128;
+            // columns that are not there repeat the last one; their products are not stored
+            const uint16_t* xk[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) xk[n] = xs + min(8 * n + g, cols - 1) * pitch + 8 * t - u0 * 128;
             while (unit < u1) {
 #pragma unroll
                 for (int d = 0; d < D; ++d) {
@@ -371,23 +375,16 @@ __global__ void __launch_bounds__(32 * kWarps, 2) k_q4_rows(RowsParams p) {
                         for (int r = 0; r < RBW; ++r) {
                             const uint4 c = cd[d][r][i >> 1];
                             const uint32_t w0 = (i & 1) ? c.z : c.x, w1 = (i & 1) ? c.w : c.y;
-#pragma unroll
-                            for (int s = 0; s < 2; ++s) {
-                                a[r][s][0] = code_pair<BF16>(w0, 2 * s);
-                                a[r][s][1] = code_pair<BF16>(w1, 2 * s);
-                                a[r][s][2] = code_pair<BF16>(w0, 2 * s + 1);
-                                a[r][s][3] = code_pair<BF16>(w1, 2 * s + 1);
-                            }
+                            code_pairs<BF16>(w0, a[r][0]);
+                            code_pairs<BF16>(w1, a[r][1]);
                         }
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            uint4 x = make_uint4(0, 0, 0, 0);
-                            if (8 * n + g < cols)
-                                x = *reinterpret_cast<const uint4*>(xk + 8 * n * pitch + unit * 128 + 32 * i);
+                            const uint4 x = *reinterpret_cast<const uint4*>(xk[n] + unit * 128 + 32 * i);
 #pragma unroll
                             for (int r = 0; r < RBW; ++r) {
-                                mma16816<BF16>(tmp[r][n], a[r][0][0], a[r][0][1], a[r][0][2], a[r][0][3], x.x, x.y);
-                                mma16816<BF16>(tmp[r][n], a[r][1][0], a[r][1][1], a[r][1][2], a[r][1][3], x.z, x.w);
+                                mma16816<BF16>(tmp[r][n], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], x.x, x.y);
+                                mma16816<BF16>(tmp[r][n], a[r][0][2], a[r][1][2], a[r][0][3], a[r][1][3], x.z, x.w);
                             }
                         }
                         if (i % FLUSH == FLUSH - 1)
@@ -433,7 +430,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) k_q4_rows(RowsParams p) {
                         const float* q = red + (k * COLS + m * SL + s) * ROWS + row;
                         y += csize > 1 ? ld_cluster(q, c) : *q;
                     }
-            if (n < p.N) static_cast<T*>(p.C)[(size_t)(c0 + m) * p.ldc + n] = from_float<T>(y);
+            if (n < p.N) static_cast<T*>(p.C)[(size_t)(c0 + m) * p.ldc + n] = from_float<T>(y * code_unit<BF16>());
         }
         // the next pass, or the exit, waits for the others' reads
         if (csize > 1) cluster_sync();
@@ -441,24 +438,24 @@ __global__ void __launch_bounds__(32 * kWarps, 2) k_q4_rows(RowsParams p) {
     }
 }
 
-template <typename T, int NT, int WR, int RBW, int D, int GROUP>
+template <typename T, int NT, int WR, int RBW, int D, int CTAS, int GROUP>
 int launch_rows_g(RowsParams p, int num_sms, cudaStream_t st) {
     constexpr int SL = sizeof(T) == 4 ? 3 : 1;
     constexpr int STEP = kWarps / WR * D * 128;                // values of K that the warps hold in flight
     const long groups = (p.l.nb + WR * RBW - 1) / (WR * RBW);
     const int experts = p.offsets ? std::min(p.E, p.R) : 1;
-    // K split over a cluster while the CTAs do not fill the GPU twice and each keeps a step of the warps
+    // K split over a cluster while all CTAs are resident at once and each keeps a step of its warps
     int ck = 1;
-    while (ck < 8 && groups * experts * ck < 2L * num_sms && p.K >= 2L * ck * STEP) ck *= 2;
+    while (ck < 8 && groups * experts * ck * 2 <= (long)CTAS * num_sms && p.K >= 2L * ck * STEP) ck *= 2;
     p.kspan = (int)(((p.K + ck - 1) / ck + 127) / 128 * 128);
     ck = (int)((p.K + p.kspan - 1) / p.kspan);
     const int cols = SL * std::min(p.R, 8 * NT / SL);
-    const int most = std::max(STEP, (96 * 1024 / (2 * cols) - 32) / STEP * STEP);
+    const int most = std::max(STEP, (196 * 1024 / CTAS / (2 * cols) - 32) / STEP * STEP);
     p.kstage = std::min(p.kspan, most);
     p.vec = (reinterpret_cast<uintptr_t>(p.A) & 15) == 0 && (p.lda * sizeof(T)) % 16 == 0;
     const size_t smem = std::max((size_t)cols * (p.kstage + 32) * 2,
                                  (size_t)(kWarps / WR) * WR * RBW * 16 * 8 * NT * 4);
-    auto kern = k_q4_rows<T, NT, WR, RBW, D, GROUP>;
+    auto kern = k_q4_rows<T, NT, WR, RBW, D, CTAS, GROUP>;
     static OncePerDevice once;
     const int e0 = once([&] { return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem); });
     if (e0) return e0;
@@ -481,12 +478,12 @@ int launch_rows_g(RowsParams p, int num_sms, cudaStream_t st) {
     return (int)cudaGetLastError();
 }
 
-template <typename T, int NT, int WR, int RBW, int D>
+template <typename T, int NT, int WR, int RBW, int D, int CTAS>
 int launch_rows_n(const RowsParams& p, int group, int num_sms, cudaStream_t st) {
     switch (group) {
-        case 32: return launch_rows_g<T, NT, WR, RBW, D, 32>(p, num_sms, st);
-        case 64: return launch_rows_g<T, NT, WR, RBW, D, 64>(p, num_sms, st);
-        default: return launch_rows_g<T, NT, WR, RBW, D, 128>(p, num_sms, st);
+        case 32: return launch_rows_g<T, NT, WR, RBW, D, CTAS, 32>(p, num_sms, st);
+        case 64: return launch_rows_g<T, NT, WR, RBW, D, CTAS, 64>(p, num_sms, st);
+        default: return launch_rows_g<T, NT, WR, RBW, D, CTAS, 128>(p, num_sms, st);
     }
 }
 
@@ -494,12 +491,12 @@ template <typename T>
 int launch_rows_t(const RowsParams& p, int group, int num_sms, cudaStream_t st) {
     const int experts = p.offsets ? std::min(p.E, p.R) : 1;
     const long cols = (long)((p.R + experts - 1) / experts) * (sizeof(T) == 4 ? 3 : 1);
-    if (cols <= 3) return launch_rows_n<T, 1, 1, 1, 4>(p, group, num_sms, st);
-    if (cols <= 8) return launch_rows_n<T, 1, 4, 1, 4>(p, group, num_sms, st);
-    if (cols <= 16) return launch_rows_n<T, 2, 4, 1, 4>(p, group, num_sms, st);
-    if (cols <= 24) return launch_rows_n<T, 3, 4, 2, 1>(p, group, num_sms, st);
-    if (cols <= 32) return launch_rows_n<T, 4, 4, 1, 2>(p, group, num_sms, st);
-    return launch_rows_n<T, 6, 4, 1, 2>(p, group, num_sms, st);
+    if (cols <= 3) return launch_rows_n<T, 1, 1, 1, 2, 4>(p, group, num_sms, st);
+    if (cols <= 8) return launch_rows_n<T, 1, 4, 1, 2, 4>(p, group, num_sms, st);
+    if (cols <= 16) return launch_rows_n<T, 2, 4, 1, 2, 3>(p, group, num_sms, st);
+    if (cols <= 24) return launch_rows_n<T, 3, 4, 2, 1, 2>(p, group, num_sms, st);
+    if (cols <= 32) return launch_rows_n<T, 4, 4, 2, 1, 2>(p, group, num_sms, st);
+    return launch_rows_n<T, 6, 4, 1, 2, 2>(p, group, num_sms, st);
 }
 
 }  // namespace

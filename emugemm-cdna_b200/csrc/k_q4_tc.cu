@@ -340,13 +340,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
                         const uint32_t w0 = odd ? hi : lo, w1 = odd ? lo : hi;
                         const int c0 = odd ? 4 + t4 : t4, c1 = c0 ^ 4;
                         uint8_t* o = st + (r * 16 + g + 8 * half) * 128;
-                        uint4 v;
-                        v.x = code_pair<BF16>(w0, 0); v.y = code_pair<BF16>(w0, 1);
-                        v.z = code_pair<BF16>(w0, 2); v.w = code_pair<BF16>(w0, 3);
-                        *reinterpret_cast<uint4*>(o + ((c0 ^ g) << 4)) = v;
-                        v.x = code_pair<BF16>(w1, 0); v.y = code_pair<BF16>(w1, 1);
-                        v.z = code_pair<BF16>(w1, 2); v.w = code_pair<BF16>(w1, 3);
-                        *reinterpret_cast<uint4*>(o + ((c1 ^ g) << 4)) = v;
+                        uint32_t v[4];
+                        code_pairs<BF16>(w0, v);
+                        *reinterpret_cast<uint4*>(o + ((c0 ^ g) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+                        code_pairs<BF16>(w1, v);
+                        *reinterpret_cast<uint4*>(o + ((c1 ^ g) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
                     }
                 }
                 fence_proxy_async_smem();
@@ -407,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
                 const int rows = tl.m1 - tl.m0 - half * H;
 #pragma unroll
                 for (int j = 0; j < H; ++j)
-                    if (j < rows) c[(size_t)j * p.ldc] = from_float<T>(sum[j]);
+                    if (j < rows) c[(size_t)j * p.ldc] = from_float<T>(sum[j] * code_unit<BF16>());
             }
         }
         if (!ok && lane == 0) abort_pair(ctl, peer);
