@@ -12,94 +12,137 @@ using namespace q4;
 
 // ------------------------------------------------------------------------------------------------- pack and unpack
 // s = bf16(fp32(max|w| / 7)) of a group, q = w / s rounded to the nearest integer (even on a tie), at most 7 away.
-// The quotient in FP32 can round onto a tie that w / s itself is not on, so q is checked with the residual w - q s:
-// |w| <= 7.1 s, so it has at most 24 significant bits where it matters and fmaf gives it exactly.
-// s below 2^-100: w and s times 2^64 first, so that 1 / s and s / 2 are normal floats; the quotient is the same.
-__device__ __forceinline__ int quantise(float w, float s, float inv) {
-    float q = rintf(w * inv);
-    const float r = fmaf(-q, s, w), h = 0.5f * s;
+// w * (1 / s) in FP32 can round onto or across a tie that w / s itself is not on, so q is checked with the residual
+// w - q s, which fmaf gives exactly where it matters (|w| <= 7.1 s: at most 24 significant bits at half a step).
+struct Scale {
+    float s, inv, half;     // the scale and its half times up, 1 / (scale * up)
+    float up;               // 2^64 for groups below 2^-90: of their scales half and inverse would not be normal floats
+    uint32_t bits;          // bf16
+    bool slow;              // values may be more than 7.5 scales away, or there is nothing to divide by
+    bool none;              // the group reads as zeros, or as NaN
+};
+// m / 7 rounded to the nearest float, m normal with m / 7 normal: the product with the rounded reciprocal, corrected by its
+// exact residual (Markstein's division step; 1 / 7 is the correctly rounded reciprocal it asks for).
+__device__ __forceinline__ float seventh(float m) {
+    const float y = 1.f / 7.f, q = m * y;
+    return fmaf(fmaf(-7.f, q, m), y, q);
+}
+__device__ __forceinline__ Scale scale_of(unsigned absmax_bits) {   // Inf and NaN compare above every number
+    Scale c;
+    const float m = __uint_as_float(absmax_bits);
+    c.slow = !(m >= 0x1p-90f) || absmax_bits >= 0x7f800000u;
+    if (!c.slow) {
+        c.none = false;
+        c.up = 1.f;
+        c.s = __bfloat162float(__float2bfloat16_rn(seventh(m)));
+        c.bits = __float_as_uint(c.s) >> 16;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(c.inv) : "f"(c.s));   // the codes are checked by their residuals
+    } else {
+        const bool bad = absmax_bits >= 0x7f800000u;
+        const float s = bad ? __uint_as_float(0x7fc00000u) : __bfloat162float(__float2bfloat16_rn(__fdiv_rn(m, 7.f)));
+        c.bits = __float_as_uint(s) >> 16;
+        c.none = bad || s == 0.f;
+        c.up = 0x1p64f;
+        c.s = s * c.up;
+        c.inv = 1.f / c.s;
+    }
+    c.half = 0.5f * c.s;
+    return c;
+}
+__device__ __forceinline__ uint32_t code_slow(float w, const Scale& c) {   // q + 8
+    if (c.none) return 8u;
+    w *= c.up;
+    float q = rintf(w * c.inv);
+    const float r = fmaf(-q, c.s, w);
     const bool odd = ((int)q) & 1;
-    if (r > h || (r == h && odd)) q += 1.f;
-    else if (r < -h || (r == -h && odd)) q -= 1.f;
-    return (int)fminf(fmaxf(q, -7.f), 7.f);
+    if (r > c.half || (r == c.half && odd)) q += 1.f;
+    else if (r < -c.half || (r == -c.half && odd)) q -= 1.f;
+    return (uint32_t)((int)fminf(fmaxf(q, -7.f), 7.f) + 8);
+}
+// q + 8 in the low four bits of w / s + 1.5 * 2^23 + 8; `off` grows to the largest residual seen: at or beyond half a
+// step the value needs code_exact.
+__device__ __forceinline__ uint32_t code_fast(float w, const Scale& c, float& off) {
+    const float t = fmaf(w, c.inv, 12582920.f);
+    off = fmaxf(off, fabsf(fmaf(-(t - 12582920.f), c.s, w)));
+    return __float_as_uint(t) & 15u;
+}
+// The same with the step towards the residual where it is beyond half a step, or half a step of an odd q: for the
+// FP32 words that code_fast finds one in (very rarely), and for 16-bit weights, where ties are common.
+__device__ __forceinline__ uint32_t code_exact(float w, const Scale& c) {
+    const float t = fmaf(w, c.inv, 12582920.f);
+    const float r = fmaf(-(t - 12582920.f), c.s, w);
+    const uint32_t u = __float_as_uint(t);
+    const bool step = fabsf(r) > c.half || (fabsf(r) == c.half && (u & 1u));
+    return (u + (step ? (r > 0.f ? 1u : ~0u) : 0u)) & 15u;
 }
 
-// One warp per tile pair: 16 rows x 128 values of K (two tiles, 4, 2 or 1 groups per row). Lane (g, t) reads rows g and
-// g + 8 at k = 32i + 8t .. +7 (i = 0..3): the values its own words of the two tiles hold. A group of 32 is then one i of
-// four lanes, so the group maximum is two shuffles, for groups of 64 and 128 after combining i pairwise in registers.
-// Bound: the read of W (4 or 2 bytes a value against half a byte written).
+// W on 16-byte boundaries: one warp per 16 rows x 128 values of K. Lane (g, t) reads rows g and g + 8 at k = 32i + 8t ..
+// +7 (i = 0..3): the values its own words of the two tiles hold. A group of 32 is one i of four lanes, so the group
+// maximum is two shuffles, for groups of 64 and 128 after combining i in registers. Bound: the read of W.
 template <typename T, int GROUP>
-__global__ void __launch_bounds__(256) k_q4_pack(const T* __restrict__ W, long ldw, int E, int N, long K, Layout l,
-                                                 uint8_t* __restrict__ packed, int vec) {
+__global__ void __launch_bounds__(256, 4) k_q4_pack(const T* __restrict__ W, long ldw, int E, int N, long K, Layout l,
+                                                 uint8_t* __restrict__ packed) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const long kp = (l.kb + 1) / 2;
     const long units = (long)E * l.nb * kp;
-    uint16_t* scales = reinterpret_cast<uint16_t*>(packed + l.scales_at);
+    constexpr int PER = GROUP / 32;   // values of i per group
+    uint32_t* scales = reinterpret_cast<uint32_t*>(packed + l.scales_at);
     for (long u = (long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (long)gridDim.x * 8) {
-        const long k128 = u % kp, b = u / kp;     // b = expert * nb + row block
+        const long b = u / kp, k128 = u - b * kp;     // b = expert * nb + row block
         const long e = b / l.nb;
-        const int n0 = (int)(b % l.nb) * 16;
-        float v[2][32];
+        const int n0 = (int)(b - e * l.nb) * 16;
+        uint32_t word[2][4], sc[2][4 / PER];          // [half of the rows]
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int n = n0 + g + 8 * half;
             const T* row = W + ((size_t)e * N + n) * ldw;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const long k = k128 * 128 + 32 * i + 8 * t;
-                float* x = v[half] + 8 * i;
-                if (n < N && vec && k + 8 <= K) {
-                    if (sizeof(T) == 4) {
-                        const float4 a = *reinterpret_cast<const float4*>(row + k);
-                        const float4 c = *reinterpret_cast<const float4*>(row + k + 4);
-                        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-                        x[4] = c.x; x[5] = c.y; x[6] = c.z; x[7] = c.w;
+            for (int gi = 0; gi < 4 / PER; ++gi) {
+                float v[PER][8];
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const long k = k128 * 128 + GROUP * gi + 32 * i + 8 * t;
+                    if (n < N && k + 8 <= K) {
+                        if (sizeof(T) == 4) {
+                            *reinterpret_cast<float4*>(v[i]) = __ldg(reinterpret_cast<const float4*>(row + k));
+                            *reinterpret_cast<float4*>(v[i] + 4) = __ldg(reinterpret_cast<const float4*>(row + k) + 1);
+                        } else {
+                            const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + k));
+                            const T* p = reinterpret_cast<const T*>(&a);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) v[i][j] = to_float<T>(p[j]);
+                        }
                     } else {
-                        const uint4 a = *reinterpret_cast<const uint4*>(row + k);
-                        const T* p = reinterpret_cast<const T*>(&a);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) x[j] = to_float<T>(p[j]);
+                        for (int j = 0; j < 8; ++j) v[i][j] = (n < N && k + j < K) ? to_float<T>(row[k + j]) : 0.f;
                     }
-                } else {
+                }
+                unsigned m = 0;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = (n < N && k + j < K) ? to_float<T>(row[k + j]) : 0.f;
+                for (int i = 0; i < PER; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[i][j]) & 0x7fffffffu);
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                const Scale c = scale_of(m);
+                sc[half][gi] = n < N ? c.bits : 0u;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    float off = 0.f;
+                    uint32_t w = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        w |= (sizeof(T) == 4 ? code_fast(v[i][j], c, off) : code_exact(v[i][j], c)) << (4 * (j / 2 + 4 * (j & 1)));
+                    if (c.slow || off >= c.half) {
+                        w = 0;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            w |= (c.slow ? code_slow(v[i][j], c) : code_exact(v[i][j], c)) << (4 * (j / 2 + 4 * (j & 1)));
+                    }
+                    word[half][gi * PER + i] = w;
                 }
             }
         }
-        uint32_t word[2][4];   // [half of the rows][i]
-        constexpr int PER = GROUP / 32;   // values of i per group
-        float sc[2][4 / PER];
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int gi = 0; gi < 4 / PER; ++gi) {
-                // the maximum of the magnitudes' bits, in which Inf and NaN come out above every number
-                unsigned m = 0;
-#pragma unroll
-                for (int j = 0; j < 8 * PER; ++j)
-                    m = max(m, __float_as_uint(v[half][8 * PER * gi + j]) & 0x7fffffffu);
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                const bool bad = m >= 0x7f800000u;
-                float s = bad ? __uint_as_float(0x7fc00000u)
-                              : __bfloat162float(__float2bfloat16_rn(__fdiv_rn(__uint_as_float(m), 7.f)));
-                sc[half][gi] = s;
-                const bool tiny = s < 0x1p-100f;
-                const float up = tiny ? 0x1p64f : 1.f;
-                const float su = s * up, inv = 1.f / su;
-                const bool none = bad || s == 0.f;
-#pragma unroll
-                for (int ii = 0; ii < PER; ++ii) {
-                    const int i = gi * PER + ii;
-                    uint32_t w = 0;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int q = none ? 0 : quantise(v[half][8 * i + j] * up, su, inv);
-                        w |= (uint32_t)(q + 8) << (4 * (j / 2 + 4 * (j & 1)));
-                    }
-                    word[half][i] = w;
-                }
-            }
         uint4* tile = reinterpret_cast<uint4*>(packed) + (size_t)(b * l.kb + 2 * k128) * 32 + lane;
         tile[0] = make_uint4(word[0][0], word[1][0], word[0][1], word[1][1]);
         if (2 * k128 + 1 < l.kb) tile[32] = make_uint4(word[0][2], word[1][2], word[0][3], word[1][3]);
@@ -107,46 +150,124 @@ __global__ void __launch_bounds__(256) k_q4_pack(const T* __restrict__ W, long l
 #pragma unroll
             for (int gi = 0; gi < 4 / PER; ++gi) {
                 const long kg = k128 * (4 / PER) + gi;
-                if (kg < l.groups) {
-                    const uint32_t lo = n0 + g < N ? __float_as_uint(sc[0][gi]) >> 16 : 0u;
-                    const uint32_t hi = n0 + g + 8 < N ? __float_as_uint(sc[1][gi]) & 0xffff0000u : 0u;
-                    reinterpret_cast<uint32_t*>(scales)[((size_t)b * l.groups + kg) * 8 + g] = lo | hi;
-                }
+                if (kg < l.groups) scales[((size_t)b * l.groups + kg) * 8 + g] = sc[0][gi] | (sc[1][gi] << 16);
             }
         }
     }
 }
 
-// W = s q in FP32 (8 + 3 significant bits: exact). One warp per tile; bound by the write.
-__global__ void __launch_bounds__(256) k_q4_unpack(const uint8_t* __restrict__ packed, int E, int N, long K, int group,
-                                                   Layout l, float* __restrict__ W, long ldw, int vec) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint16_t* scales = reinterpret_cast<const uint16_t*>(packed + l.scales_at);
-    const long units = (long)E * l.nb * l.kb;
+// W on other boundaries: one warp per 128 values of rows r and r + 8 of a row block, a lane per value of each 32, so that
+// the loads stay contiguous whatever the alignment; the group maximum is one warp reduction per 32 values, and a word is
+// put together by three shuffles among its eight lanes. (With the mapping above and 2-byte loads 16 bytes apart,
+// 5 x 1000 x 1111 bf16 weights took 61 us with their read back.)
+template <typename T, int GROUP>
+__global__ void __launch_bounds__(256) k_q4_pack_rows(const T* __restrict__ W, long ldw, int E, int N, long K, Layout l,
+                                                      uint8_t* __restrict__ packed) {
+    const int lane = threadIdx.x & 31;
+    const long kp = (l.kb + 1) / 2, rows = l.nb * 8;
+    const long units = (long)E * rows * kp;
+    constexpr int PER = GROUP / 32;
+    uint2* codes = reinterpret_cast<uint2*>(packed);
+    uint32_t* scales = reinterpret_cast<uint32_t*>(packed + l.scales_at);
     for (long u = (long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (long)gridDim.x * 8) {
-        const long kb = u % l.kb, b = u / l.kb, e = b / l.nb;
-        const int n0 = (int)(b % l.nb) * 16;
-        const uint4 c = reinterpret_cast<const uint4*>(packed)[(size_t)u * 32 + lane];
+        const long rr = u / kp, k128 = u - rr * kp;
+        const long b = rr >> 3, e = b / l.nb;
+        const int r = (int)(rr & 7), n = (int)(b - e * l.nb) * 16 + r;
+        const T* row = W + ((size_t)e * N + n) * ldw + k128 * 128 + lane;
+        const long left = K - k128 * 128 - lane;
+        float v[2][4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[half][i] = n + 8 * half < N && 32 * i < left ? to_float<T>(row[8 * half * ldw + 32 * i]) : 0.f;
+        uint32_t word[2][4];
+#pragma unroll
+        for (int gi = 0; gi < 4 / PER; ++gi) {
+            uint32_t sc[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                unsigned m = 0;
+#pragma unroll
+                for (int i = gi * PER; i < (gi + 1) * PER; ++i) m = max(m, __float_as_uint(v[half][i]) & 0x7fffffffu);
+                const Scale c = scale_of(__reduce_max_sync(0xffffffffu, m));
+                sc[half] = n + 8 * half < N ? c.bits : 0u;
+#pragma unroll
+                for (int i = gi * PER; i < (gi + 1) * PER; ++i) {
+                    const int j = lane & 7;
+                    uint32_t w = (c.slow ? code_slow(v[half][i], c) : code_exact(v[half][i], c)) << (4 * (j / 2 + 4 * (j & 1)));
+                    w |= __shfl_xor_sync(0xffffffffu, w, 1);
+                    w |= __shfl_xor_sync(0xffffffffu, w, 2);
+                    w |= __shfl_xor_sync(0xffffffffu, w, 4);
+                    word[half][i] = w;
+                }
+            }
+            const long kg = k128 * (4 / PER) + gi;
+            if (lane == 0 && kg < l.groups) scales[((size_t)b * l.groups + kg) * 8 + r] = sc[0] | (sc[1] << 16);
+        }
+        if ((lane & 7) == 0)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const long kb = 2 * k128 + (i >> 1);
+                if (kb < l.kb) codes[(size_t)(b * l.kb + kb) * 64 + (r * 4 + (lane >> 3)) * 2 + (i & 1)] = make_uint2(word[0][i], word[1][i]);
+            }
+    }
+}
+
+// W = s q in FP32 (8 + 3 significant bits: exact). One warp per tile: the tile comes in as one 512-byte access and goes out
+// as rows, their words and scales handed to the lanes by shuffles. Bound: the write. VEC: rows on 16-byte boundaries, a
+// lane writes four values and a warp two rows at a time; else a value per lane, so that 32 stay one 128-byte access at any
+// alignment (70 us against 45 for 8192 x 8192).
+template <bool VEC>
+__global__ void __launch_bounds__(256) k_q4_unpack(const uint8_t* __restrict__ packed, int E, int N, long K, int group,
+                                                   Layout l, float* __restrict__ W, long ldw) {
+    const int lane = threadIdx.x & 31, g = lane >> 2;
+    const uint32_t* scales = reinterpret_cast<const uint32_t*>(packed + l.scales_at);
+    const long units = (long)E * l.nb * l.kb;
+    // 2^23 + u - (2^23 + 8)
+    auto value = [](uint32_t u) { return __uint_as_float((u & 15u) | 0x4b000000u) - 8388616.f; };
+    for (long u = (long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (long)gridDim.x * 8) {
+        const long b = u / l.kb, kb = u - b * l.kb, e = b / l.nb;
+        const int n0 = (int)(b - e * l.nb) * 16;
+        const uint4 c = __ldg(reinterpret_cast<const uint4*>(packed) + (size_t)u * 32 + lane);
         const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+        uint32_t sw[2];   // the scales of rows g and g + 8 for the two halves of the tile
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int n = n0 + g + 8 * (i & 1);
-            const long k = kb * 64 + 32 * (i >> 1) + 8 * t;
-            if (n >= N || k >= K) continue;
-            const float s = __uint_as_float(
-                (uint32_t)scales[(((size_t)b * l.groups + k / group) * 8 + g) * 2 + (i & 1)] << 16);
-            float x[8];
+        for (int h = 0; h < 2; ++h)
+            sw[h] = kb * 64 + 32 * h < K ? __ldg(scales + ((size_t)b * l.groups + (kb * 64 + 32 * h) / group) * 8 + g) : 0u;
+        if (VEC) {
+            // lane: row 2j + (lane >> 4), values 4 (lane & 15) .. + 3, half a word
+            const int k = 4 * (lane & 15), h = k >> 5, from = (k >> 3) & 3, shift = 8 * ((k >> 2) & 1);
+            float* out = W + ((size_t)e * N + n0) * ldw + kb * 64 + k;
+            const long left = K - kb * 64 - k;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                x[j] = s * (float)((int)((w[i] >> (4 * (j / 2 + 4 * (j & 1)))) & 15u) - 8);
-            float* row = W + ((size_t)e * N + n) * ldw + k;
-            if (vec && k + 8 <= K) {
-                reinterpret_cast<float4*>(row)[0] = make_float4(x[0], x[1], x[2], x[3]);
-                reinterpret_cast<float4*>(row)[1] = make_float4(x[4], x[5], x[6], x[7]);
-            } else {
+            for (int j = 0; j < 8; ++j) {
+                const int row = 2 * j + (lane >> 4), hi = j >> 2;
+                const uint32_t w0 = __shfl_sync(0xffffffffu, w[hi], (row & 7) * 4 + from);
+                const uint32_t w1 = __shfl_sync(0xffffffffu, w[2 + hi], (row & 7) * 4 + from);
+                const uint32_t s0 = __shfl_sync(0xffffffffu, sw[0], (row & 7) * 4);
+                const uint32_t s1 = __shfl_sync(0xffffffffu, sw[1], (row & 7) * 4);
+                const uint32_t word = (h ? w1 : w0) >> shift, sp = h ? s1 : s0;
+                const float s = hi ? bf16_hi(sp) : bf16_lo(sp);
+                if (n0 + row < N && left > 0)
+                    *reinterpret_cast<float4*>(out + (size_t)row * ldw) =
+                        make_float4(s * value(word), s * value(word >> 16), s * value(word >> 4), s * value(word >> 20));
+            }
+        } else {
+            const int shift = 4 * ((lane & 7) / 2 + 4 * (lane & 1));
+            float* out = W + ((size_t)e * N + n0) * ldw + kb * 64 + lane;
+            const long left = K - kb * 64 - lane;
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (k + j < K) row[j] = x[j];
+            for (int i = 0; i < 4; ++i) {                // word i: rows 8 (i & 1) .. +7, half i >> 1 of the tile
+                const int h = i >> 1;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const uint32_t word = __shfl_sync(0xffffffffu, w[i], r * 4 + (lane >> 3));
+                    const uint32_t sp = __shfl_sync(0xffffffffu, sw[h], r * 4);
+                    const int n = 8 * (i & 1) + r;
+                    if (n0 + n < N && 32 * h < left)
+                        out[(size_t)n * ldw + 32 * h] = ((i & 1) ? bf16_hi(sp) : bf16_lo(sp)) * value(word >> shift);
+                }
             }
         }
     }
@@ -503,19 +624,28 @@ int launch_rows_t(const RowsParams& p, int group, int num_sms, cudaStream_t st) 
 
 size_t q4_bytes(int E, int N, long K, int group) { return layout(E, N, K, group).bytes; }
 
-template <typename T>
-static int pack_t(const void* W, long ldw, int E, int N, long K, int group, void* packed, int num_sms, cudaStream_t st) {
-    const Layout l = layout(E, N, K, group);
-    const long units = (long)E * l.nb * ((l.kb + 1) / 2);
-    const int vec = (reinterpret_cast<uintptr_t>(W) & 15) == 0 && (ldw * sizeof(T)) % 16 == 0;
-    const int grid = (int)std::min((units + 7) / 8, 8L * num_sms);
-    const T* w = static_cast<const T*>(W);
-    uint8_t* o = static_cast<uint8_t*>(packed);
-    if (group == 32) k_q4_pack<T, 32><<<grid, 256, 0, st>>>(w, ldw, E, N, K, l, o, vec);
-    else if (group == 64) k_q4_pack<T, 64><<<grid, 256, 0, st>>>(w, ldw, E, N, K, l, o, vec);
-    else k_q4_pack<T, 128><<<grid, 256, 0, st>>>(w, ldw, E, N, K, l, o, vec);
+template <typename T, int GROUP>
+static int pack_g(const T* W, long ldw, int E, int N, long K, uint8_t* packed, int num_sms, cudaStream_t st) {
+    const Layout l = layout(E, N, K, GROUP);
+    const long pairs = (long)E * l.nb * ((l.kb + 1) / 2);
+    if ((reinterpret_cast<uintptr_t>(W) & 15) == 0 && (ldw * sizeof(T)) % 16 == 0) {
+        const int grid = (int)std::min((pairs + 7) / 8, 16L * num_sms);
+        k_q4_pack<T, GROUP><<<grid, 256, 0, st>>>(W, ldw, E, N, K, l, packed);
+    } else {
+        const int grid = (int)std::min(pairs, 32L * num_sms);
+        k_q4_pack_rows<T, GROUP><<<grid, 256, 0, st>>>(W, ldw, E, N, K, l, packed);
+    }
     count_launch();
     return (int)cudaGetLastError();
+}
+
+template <typename T>
+static int pack_t(const void* W, long ldw, int E, int N, long K, int group, void* packed, int num_sms, cudaStream_t st) {
+    const T* w = static_cast<const T*>(W);
+    uint8_t* o = static_cast<uint8_t*>(packed);
+    if (group == 32) return pack_g<T, 32>(w, ldw, E, N, K, o, num_sms, st);
+    if (group == 64) return pack_g<T, 64>(w, ldw, E, N, K, o, num_sms, st);
+    return pack_g<T, 128>(w, ldw, E, N, K, o, num_sms, st);
 }
 
 int launch_q4_pack(const void* W, long ldw, int dtype, int E, int N, long K, int group, void* packed, int num_sms,
@@ -530,10 +660,10 @@ int launch_q4_unpack(const void* packed, int E, int N, long K, int group, float*
                      void* stream) {
     const Layout l = layout(E, N, K, group);
     const long units = (long)E * l.nb * l.kb;
-    const int vec = (reinterpret_cast<uintptr_t>(W) & 15) == 0 && ldw % 4 == 0;
-    const int grid = (int)std::min((units + 7) / 8, 16L * num_sms);
-    k_q4_unpack<<<grid, 256, 0, (cudaStream_t)stream>>>(static_cast<const uint8_t*>(packed), E, N, K, group, l, W, ldw,
-                                                        vec);
+    const int grid = (int)std::min((units + 7) / 8, 32L * num_sms);
+    const bool vec = (reinterpret_cast<uintptr_t>(W) & 15) == 0 && ldw % 4 == 0 && K % 4 == 0;
+    auto kern = vec ? k_q4_unpack<true> : k_q4_unpack<false>;
+    kern<<<grid, 256, 0, (cudaStream_t)stream>>>(static_cast<const uint8_t*>(packed), E, N, K, group, l, W, ldw);
     count_launch();
     return (int)cudaGetLastError();
 }

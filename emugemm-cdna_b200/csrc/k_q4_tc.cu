@@ -48,7 +48,10 @@ struct Cfg {
     static constexpr int STAGES = FIT < kMaxStages ? FIT : kMaxStages;
     static constexpr int BUFS = 512 / TN < kMaxBufs ? 512 / TN : kMaxBufs;
     static constexpr int SMEM = STAGES * STAGE + kSmemFixed;
-    static_assert(STAGES >= 3 && SMEM <= kSmemMax, "shared memory");
+    static_assert(SMEM <= kSmemMax, "shared memory");
+    // A wait tells apart only two neighbouring phases of a barrier: when a converter warp comes to a stage, the use before
+    // the last must be known to be over. It knows of the panels up to STAGES before its previous one, kConvPairs back.
+    static_assert(STAGES >= kConvPairs, "phases of the empty barriers");
     static_assert(PANEL_B % 1024 == 0, "swizzle atoms");
 };
 

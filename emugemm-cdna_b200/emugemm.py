@@ -182,6 +182,7 @@ def _ptr(x) -> int:
 
 
 _dtype_codes: dict = {}   # tensor dtype -> emu_dtype_t
+_dtype_names: dict = {}   # tensor dtype -> its name (str of a dtype takes longer than the rest of a call's checks)
 
 
 def _dtype(dtype, *xs) -> int:
@@ -205,9 +206,14 @@ def _dtype(dtype, *xs) -> int:
 def _typed(x, name: str) -> int:
     """Pointer of x, which, if a tensor, must have the dtype `name` (ValueError)."""
     d = getattr(x, "dtype", None)
-    if d is not None and str(d) != name:
+    if d is None:
+        return _ptr(x)
+    known = _dtype_names.get(d)
+    if known is None:
+        known = _dtype_names[d] = str(d)
+    if known != name:
         raise ValueError(f"expected a {name} tensor, got {d}")
-    return _ptr(x)
+    return x.data_ptr()
 
 
 def q4_bytes(E: int, N: int, K: int, group: int) -> int:
