@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(256) k_q4_unpack(const uint8_t* __restrict__ p
 // of K in turn, their sums are added in order, and where there are few row blocks a cluster of CTAs splits K and adds
 // its parts over distributed shared memory.
 constexpr int kWarps = 8;
-constexpr int kRowsSmem = 100 * 1024;
+constexpr int kRowsSmem = 110 * 1024;
 
 struct RowsParams {
     const void* A; long lda;
@@ -312,6 +312,21 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
                      "{%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <bool BF16>
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {   // d = a * b
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ uint4 ld_codes(const uint4* p) {
@@ -368,6 +383,70 @@ __device__ __forceinline__ bool nth_expert(const int* offsets, int E, int i, int
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {   // the rest of 16 is zeroed
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// Rows of A (toks rows of `len` values) into shared memory as 16-bit columns, zeros from len to span; a warp takes 256 values
+// of a row at a time. Rows on 16-byte boundaries: 8 values per lane, 16-bit ones as asynchronous copies; others: a value
+// per lane at a time, so that the loads stay contiguous.
+template <typename T>
+__device__ __forceinline__ void stage_rows(uint16_t* xs, int pitch, const T* rows, long lda, int toks, int span, int len,
+                                           int vec) {
+    constexpr int SL = sizeof(T) == 4 ? 3 : 1;
+    const int lane = threadIdx.x & 31;
+    int m = 0, k0 = (threadIdx.x >> 5) * 256;
+    while (true) {
+        while (k0 >= span) {
+            k0 -= (span + 255) / 256 * 256;
+            if (k0 < 0) k0 = 0;
+            if (++m >= toks) return;
+        }
+        const T* row = rows + (size_t)m * lda;
+        if (vec) {
+            const int k = k0 + lane * 8, left = len - k;
+            if (k < span) {
+                if (SL == 1) {
+                    cp_async16(static_cast<uint32_t>(__cvta_generic_to_shared(xs + m * pitch + k)), left > 0 ? row + k : rows,
+                               left <= 0 ? 0 : left >= 8 ? 16 : 2 * left);
+                } else {
+                    __align__(16) float x[8];
+                    if (left >= 8) {
+                        *reinterpret_cast<float4*>(x) = __ldg(reinterpret_cast<const float4*>(row + k));
+                        *reinterpret_cast<float4*>(x + 4) = __ldg(reinterpret_cast<const float4*>(row + k) + 1);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) x[j] = j < left ? to_float<T>(row[k + j]) : 0.f;
+                    }
+                    __align__(16) uint16_t s[3][8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) slice3(x[j], s[0][j], s[1][j], s[2][j]);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i)
+                        *reinterpret_cast<uint4*>(xs + (3 * m + i) * pitch + k) = *reinterpret_cast<const uint4*>(s[i]);
+                }
+            }
+        } else {
+            T x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int k = k0 + 32 * j + lane;
+                x[j] = k < len ? row[k] : from_float<T>(0.f);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int k = k0 + 32 * j + lane;
+                if (k >= span) break;
+                if (SL == 3) {
+                    uint16_t s[3];
+                    slice3(to_float<T>(x[j]), s[0], s[1], s[2]);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) xs[(3 * m + i) * pitch + k] = s[i];
+                } else {
+                    xs[m * pitch + k] = *reinterpret_cast<const uint16_t*>(&x[j]);
+                }
+            }
+        }
+        k0 += 256 * kWarps;
+    }
 }
 
 // T: type of A and C; NT: column tiles of 8; WR: warps over row blocks; RBW: row blocks per warp; D: units of 128
@@ -440,37 +519,7 @@ __global__ void __launch_bounds__(32 * kWarps, CTAS) k_q4_rows(RowsParams p) {
             const int span = (u1 - u0) * 128;
             const long ks = kbeg + (long)u0 * 128;
             if (u0) __syncthreads();
-            for (int m = 0; m < toks; ++m) {
-                const T* row = A + (size_t)(c0 + m) * p.lda + ks;
-                const int len = (int)min((long)span, p.K - ks);
-                for (int k = threadIdx.x * 8; k < span; k += 256 * kWarps) {
-                    if (SL == 1 && p.vec) {
-                        const int left = len - k;
-                        cp_async16(static_cast<uint32_t>(__cvta_generic_to_shared(xs + m * pitch + k)),
-                                   left > 0 ? row + k : A, left <= 0 ? 0 : left >= 8 ? 16 : 2 * left);
-                        continue;
-                    }
-                    T x[8];
-                    if (p.vec && k + 8 <= len) {
-#pragma unroll
-                        for (int j = 0; j < 8 * (int)sizeof(T) / 16; ++j)
-                            reinterpret_cast<uint4*>(x)[j] = __ldg(reinterpret_cast<const uint4*>(row + k) + j);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) x[j] = k + j < len ? row[k + j] : from_float<T>(0.f);
-                    }
-                    if (SL == 3) {
-                        __align__(16) uint16_t s[3][8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) slice3(to_float<T>(x[j]), s[0][j], s[1][j], s[2][j]);
-#pragma unroll
-                        for (int q = 0; q < 3; ++q)
-                            *reinterpret_cast<uint4*>(xs + (3 * m + q) * pitch + k) = *reinterpret_cast<const uint4*>(s[q]);
-                    } else {
-                        *reinterpret_cast<uint4*>(xs + m * pitch + k) = *reinterpret_cast<const uint4*>(x);
-                    }
-                }
-            }
+            stage_rows<T>(xs, pitch, A + (size_t)c0 * p.lda + ks, p.lda, toks, span, (int)min((long)span, p.K - ks), p.vec);
             if (SL == 1) asm volatile("cp.async.wait_all;" ::: "memory");
             __syncthreads();
             // columns that are not there repeat the last one; their products are not stored
@@ -484,13 +533,6 @@ __global__ void __launch_bounds__(32 * kWarps, CTAS) k_q4_rows(RowsParams p) {
                     float tmp[RBW][NT][4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {   // 32 values of K: half i & 1 of tile i >> 1
-                        if (i % FLUSH == 0)
-#pragma unroll
-                            for (int r = 0; r < RBW; ++r)
-#pragma unroll
-                                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j) tmp[r][n][j] = 0.f;
                         uint32_t a[RBW][2][4];
 #pragma unroll
                         for (int r = 0; r < RBW; ++r) {
@@ -504,7 +546,8 @@ __global__ void __launch_bounds__(32 * kWarps, CTAS) k_q4_rows(RowsParams p) {
                             const uint4 x = *reinterpret_cast<const uint4*>(xk[n] + unit * 128 + 32 * i);
 #pragma unroll
                             for (int r = 0; r < RBW; ++r) {
-                                mma16816<BF16>(tmp[r][n], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], x.x, x.y);
+                                if (i % FLUSH == 0) mma16816_zero<BF16>(tmp[r][n], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], x.x, x.y);
+                                else mma16816<BF16>(tmp[r][n], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], x.x, x.y);
                                 mma16816<BF16>(tmp[r][n], a[r][0][2], a[r][1][2], a[r][0][3], a[r][1][3], x.z, x.w);
                             }
                         }
@@ -567,11 +610,11 @@ int launch_rows_g(RowsParams p, int num_sms, cudaStream_t st) {
     const int experts = p.offsets ? std::min(p.E, p.R) : 1;
     // K split over a cluster while all CTAs are resident at once and each keeps a step of its warps
     int ck = 1;
-    while (ck < 8 && groups * experts * ck * 2 <= (long)CTAS * num_sms && p.K >= 2L * ck * STEP) ck *= 2;
+    while (ck < 8 && groups * experts * ck * 2 <= (long)(NT == 1 && WR == 1 ? 1 : CTAS) * num_sms && p.K >= 2L * ck * STEP) ck *= 2;
     p.kspan = (int)(((p.K + ck - 1) / ck + 127) / 128 * 128);
     ck = (int)((p.K + p.kspan - 1) / p.kspan);
     const int cols = SL * std::min(p.R, 8 * NT / SL);
-    const int most = std::max(STEP, (196 * 1024 / CTAS / (2 * cols) - 32) / STEP * STEP);
+    const int most = std::max(STEP, (218 * 1024 / CTAS / (2 * cols) - 32) / STEP * STEP);
     p.kstage = std::min(p.kspan, most);
     p.vec = (reinterpret_cast<uintptr_t>(p.A) & 15) == 0 && (p.lda * sizeof(T)) % 16 == 0;
     const size_t smem = std::max((size_t)cols * (p.kstage + 32) * 2,
@@ -612,12 +655,17 @@ template <typename T>
 int launch_rows_t(const RowsParams& p, int group, int num_sms, cudaStream_t st) {
     const int experts = p.offsets ? std::min(p.E, p.R) : 1;
     const long cols = (long)((p.R + experts - 1) / experts) * (sizeof(T) == 4 ? 3 : 1);
-    if (cols <= 3) return launch_rows_n<T, 1, 1, 1, 2, 4>(p, group, num_sms, st);
-    if (cols <= 8) return launch_rows_n<T, 1, 4, 1, 2, 4>(p, group, num_sms, st);
-    if (cols <= 16) return launch_rows_n<T, 2, 4, 1, 2, 3>(p, group, num_sms, st);
-    if (cols <= 24) return launch_rows_n<T, 3, 4, 2, 1, 2>(p, group, num_sms, st);
-    if (cols <= 32) return launch_rows_n<T, 4, 4, 2, 1, 2>(p, group, num_sms, st);
-    return launch_rows_n<T, 6, 4, 1, 2, 2>(p, group, num_sms, st);
+    if (cols <= 3) return launch_rows_n<T, 1, 1, 2, 2, 2>(p, group, num_sms, st);
+    if (cols <= 8) return launch_rows_n<T, 1, 8, 2, 2, 2>(p, group, num_sms, st);
+    if (cols <= 16) return launch_rows_n<T, 2, 8, 2, 2, 2>(p, group, num_sms, st);
+    if (cols <= 24) {
+        // scales of four groups per unit and two row blocks do not fit the registers beside three column tiles
+        // (24 x 5001 x 7013, groups of 32: 23.0 against 20.8 us; 24 x 8192 x 8192, groups of 128: 19.7 against 26.0)
+        if (group == 32) return launch_rows_g<T, 3, 8, 1, 1, 3, 32>(p, num_sms, st);
+        return launch_rows_n<T, 3, 8, 2, 1, 2>(p, group, num_sms, st);
+    }
+    if (cols <= 32) return launch_rows_n<T, 4, 8, 1, 2, 2>(p, group, num_sms, st);
+    return launch_rows_n<T, 6, 8, 1, 2, 2>(p, group, num_sms, st);
 }
 
 }  // namespace
