@@ -362,21 +362,27 @@ __device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
 // Expert and rows of blockIdx.y: the i-th expert that has rows (all lanes of a warp call it; false: there is none).
 __device__ __forceinline__ bool nth_expert(const int* offsets, int E, int i, int R, int& e, int& r0, int& r1) {
     const int lane = threadIdx.x & 31;
-    for (int base = 0; base < E; base += 32) {
-        const int x = base + lane;
-        const int a = x < E ? offsets[x] : 0, b = x < E ? offsets[x + 1] : 0;
-        const unsigned some = __ballot_sync(0xffffffffu, b > a);
-        const int n = __popc(some);
-        if (i < n) {
-            unsigned m = some;
-            for (int j = 0; j < i; ++j) m &= m - 1;
-            const int src = __ffs(m) - 1;
-            e = base + src;
-            r0 = max(0, __shfl_sync(0xffffffffu, a, src));
-            r1 = min(R, __shfl_sync(0xffffffffu, b, src));   // a bad offset reads and writes no row outside of A and C
-            return true;
+    for (int base = 0; base < E; base += 128) {
+        int a[4], b[4];                          // 128 experts at a time: one wait for their offsets
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int x = base + 32 * j + lane;
+            a[j] = x < E ? __ldg(offsets + x) : 0;
+            b[j] = x < E ? __ldg(offsets + x + 1) : 0;
         }
-        i -= n;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned some = __ballot_sync(0xffffffffu, b[j] > a[j]);
+            const int n = __popc(some);
+            if (i < n) {
+                const int src = __fns(some, 0, i + 1);
+                e = base + 32 * j + src;
+                r0 = max(0, __shfl_sync(0xffffffffu, a[j], src));
+                r1 = min(R, __shfl_sync(0xffffffffu, b[j], src));   // a bad offset reads and writes no row outside of A and C
+                return true;
+            }
+            i -= n;
+        }
     }
     return false;
 }
@@ -651,11 +657,17 @@ int launch_rows_n(const RowsParams& p, int group, int num_sms, cudaStream_t st) 
     }
 }
 
+// Tiles by the columns of a pass (rows of A, three times as many for FP32). With experts: twice the mean, since rows are
+// never dealt evenly and a second pass reads the codes again; and for up to 8 columns few row blocks per CTA until the CTAs
+// fill the GPU anyway (8 tokens x 4 of 64 experts, 2048 x 4096: 23 us with 4 row blocks against 25 with 16 and 27 with 2;
+// 64 x 8 of 256, 2048 x 1024: 68 us with 4, 59 with 16).
 template <typename T>
 int launch_rows_t(const RowsParams& p, int group, int num_sms, cudaStream_t st) {
     const int experts = p.offsets ? std::min(p.E, p.R) : 1;
-    const long cols = (long)((p.R + experts - 1) / experts) * (sizeof(T) == 4 ? 3 : 1);
-    if (cols <= 3) return launch_rows_n<T, 1, 1, 2, 2, 2>(p, group, num_sms, st);
+    const long cols = (long)((p.R + experts - 1) / experts) * (sizeof(T) == 4 ? 3 : 1) * (p.offsets ? 2 : 1);
+    if (p.offsets && cols <= 8 && p.l.nb * experts < 32L * num_sms)
+        return launch_rows_n<T, 1, 2, 2, 2, 2>(p, group, num_sms, st);
+    if (!p.offsets && cols <= 3) return launch_rows_n<T, 1, 1, 2, 2, 2>(p, group, num_sms, st);
     if (cols <= 8) return launch_rows_n<T, 1, 8, 2, 2, 2>(p, group, num_sms, st);
     if (cols <= 16) return launch_rows_n<T, 2, 8, 2, 2, 2>(p, group, num_sms, st);
     if (cols <= 24) {
