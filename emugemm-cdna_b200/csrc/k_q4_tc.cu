@@ -48,7 +48,7 @@ struct Cfg {
     static constexpr int STAGES = FIT < kMaxStages ? FIT : kMaxStages;
     static constexpr int BUFS = 512 / TN < kMaxBufs ? 512 / TN : kMaxBufs;
     static constexpr int SMEM = STAGES * STAGE + kSmemFixed;
-    static_assert(SMEM <= kSmemMax, "shared memory");
+    static_assert(SMEM <= kSmemMax && TN * 128 * 4 <= STAGES * STAGE, "shared memory");
     // A wait tells apart only two neighbouring phases of a barrier: when a converter warp comes to a stage, the use before
     // the last must be known to be over. It knows of the panels up to STAGES before its previous one, kConvPairs back.
     static_assert(STAGES >= kConvPairs, "phases of the empty barriers");
@@ -75,6 +75,7 @@ struct Params {
     int R, E, N;
     int num_n;                      // 256-row tiles of the weights
     int np;                         // panels per tile (even)
+    int ks, span;                   // K splits (pairs per cluster), panels of each (even; the last may have fewer)
     int plane;                      // rows between the slices of A (SL = 3)
     unsigned* err;
 };
@@ -88,6 +89,11 @@ __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ void abort_pair(Ctl* ctl, uint32_t peer) {
     ctl->abort = 1;
     st_shared_cluster_u32(mapa_shared(smem_u32(&ctl->abort), peer), 1u);
+}
+__device__ __forceinline__ float ld_shared_cluster(const float* p, uint32_t rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+    return v;
 }
 template <int N>
 __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -156,12 +162,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Ctl* ctl = reinterpret_cast<Ctl*>(smem + ST * C_::STAGE);
     int* first = reinterpret_cast<int*>(ctl + 1);
+    float* red = reinterpret_cast<float*>(smem);   // ks > 1: [TN][128] sums of this pair's part of K, after the last product
+    constexpr int H = TN / 2;
     volatile int* abort = &ctl->abort;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_ctarank(), peer = rank ^ 1u;
+    // a cluster is one pair, or ks of them that share a tile and split its K
+    const uint32_t crank = cluster_ctarank(), peer = crank ^ 1u, lead = crank & ~1u, rank = crank & 1u;
     const bool leader = rank == 0;
-    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+    const int pair = blockIdx.x / (2 * p.ks), num_pairs = gridDim.x / (2 * p.ks);
+    const int p0 = (int)(crank >> 1) * p.span, np = min(p.np, p0 + p.span) - p0;   // panels of this pair
+    const uint16_t both = (uint16_t)(3u << lead);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; ++s) {
@@ -202,19 +213,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = ctl->tmem_base;
-    const int num_tiles = (p.offsets ? first[p.E] : (p.R + TN - 1) / TN) * p.num_n;
+    int num_tiles = (p.offsets ? first[p.E] : (p.R + TN - 1) / TN) * p.num_n;
+    if (p.ks > 1) num_tiles = min(num_tiles, num_pairs);   // one tile per cluster (more only with overlapping offsets)
 
     if (warp < 8) {
         reg_dec<kRegOther>();
         if (warp == 0 && lane == 0) {
             // ---------------- TMA producer: this CTA's half of the rows of A ----------------
-            const uint32_t lead_full0 = mapa_shared(smem_u32(&ctl->full[0]), 0);
+            const uint32_t lead_full0 = mapa_shared(smem_u32(&ctl->full[0]), lead);
             long it = 0;
             bool ok = true;
             for (int t = pair; t < num_tiles && ok; t += num_pairs) {
                 const Tile tl = tile_of<TN>(p, first, t);
                 const int row = tl.m0 + (int)rank * (TN / 2);
-                for (int k = 0; k < p.np; ++k, ++it) {
+                for (int k = 0; k < np; ++k, ++it) {
                     const int s = (int)(it % ST);
                     if (!wait(&ctl->empty[s], (uint32_t)((it / ST) & 1) ^ 1u, abort, p.err, kErrTimeoutProducer)) {
                         ok = false;
@@ -226,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
                     uint8_t* st = smem + s * C_::STAGE + kPanelA;
 #pragma unroll
                     for (int sl = 0; sl < SL; ++sl)
-                        tma_load_2d_pair(st + sl * C_::PANEL_B, &tm_x, fb, k * 64, sl * p.plane + row);
+                        tma_load_2d_pair(st + sl * C_::PANEL_B, &tm_x, fb, (p0 + k) * 64, sl * p.plane + row);
                 }
             }
             if (!ok) {
@@ -245,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
             uint32_t ph = 0, pu = 1;
             bool ok = true;
             for (int t = pair; t < num_tiles && ok; t += num_pairs) {
-                for (int k = 0; k < p.np && ok; k += PPG) {
+                for (int k = 0; k < np && ok; k += PPG) {
 #pragma unroll
                     for (int h = 0; h < PPG && ok; ++h) {
                         bool ready = wait(&ctl->full[s], ph, abort, p.err, kErrTimeoutMma);
@@ -265,8 +277,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
                                         mma_f16_ss_pair(d, a, a + (uint64_t)((kPanelA + sl * C_::PANEL_B) >> 4), kIdesc,
                                                         h != 0 || j != 0 || sl != SL - 1 ? 1u : 0u);
                                     }
-                                if (h == PPG - 1) mma_commit_pair_both(&ctl->tmem_full[u], (uint16_t)0x3);
-                                if (q == GPP - 1) mma_commit_pair_both(&ctl->empty[s], (uint16_t)0x3);
+                                if (h == PPG - 1) mma_commit_pair_both(&ctl->tmem_full[u], both);
+                                if (q == GPP - 1) mma_commit_pair_both(&ctl->empty[s], both);
                             }
                             if (h == PPG - 1 && ++u == NB) { u = 0; pu ^= 1u; }
                         }
@@ -283,8 +295,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
             // ---------------- converters: codes -> integers in the swizzled K-major operand ----------------
             // A pair of warps takes every third panel of the pair's tiles, each warp 64 of the CTA's 128 weight rows.
             const int cp = (warp - 2) >> 1, cw = warp & 1, g = lane >> 2, t4 = lane & 3;
-            const uint32_t lead_full0 = mapa_shared(smem_u32(&ctl->full[0]), 0);
-            const uint32_t lead_slot = mapa_shared(smem_u32(&ctl->sig_dst[2 * cp + cw][0]), 0);
+            const uint32_t lead_full0 = mapa_shared(smem_u32(&ctl->full[0]), lead);
+            const uint32_t lead_slot = mapa_shared(smem_u32(&ctl->sig_dst[2 * cp + cw][0]), lead);
             const uint32_t sig_src = smem_u32(&ctl->sig_src[0]);
             const uint4 none = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
             const uint4* codes = reinterpret_cast<const uint4*>(p.packed);
@@ -301,12 +313,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
             auto load = [&](uint4 (&c)[4]) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    c[r] = r < rows && k < p.l.kb ? __ldg(src + ((size_t)r * p.l.kb + k) * 32) : none;
+                    c[r] = r < rows && p0 + k < p.l.kb ? __ldg(src + ((size_t)r * p.l.kb + p0 + k) * 32) : none;
             };
             auto settle = [&]() {                  // the panel's tile, when k has run past the end of one
                 bool moved = false;
-                while (k >= p.np && t < num_tiles) {
-                    k -= p.np;
+                while (k >= np && t < num_tiles) {
+                    k -= np;
                     t += num_pairs;
                     moved = true;
                 }
@@ -364,17 +376,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
         const int sp = warp & 3, half = (warp - 8) >> 2;
         const int row_in_tile = (int)rank * 128 + sp * 32 + lane;
         const uint32_t lane_off = (uint32_t)(sp * 32) << 16;
-        const uint32_t lead_te0 = mapa_shared(smem_u32(&ctl->tmem_empty[0]), 0);
+        const uint32_t lead_te0 = mapa_shared(smem_u32(&ctl->tmem_empty[0]), lead);
         const uint16_t* scales = reinterpret_cast<const uint16_t*>(p.packed + p.l.scales_at);
-        const int groups = p.np * 64 / GROUP;              // of the padded K
-        constexpr int H = TN / 2;
+        const int g0 = p0 * 64 / GROUP, groups = np * 64 / GROUP;   // of the padded K
         long ch = 0;
         bool ok = true;
         for (int t = pair; t < num_tiles && ok; t += num_pairs) {
             const Tile tl = tile_of<TN>(p, first, t);
             const int n = tl.nb * 256 + row_in_tile;
             const bool there = n < p.N;
-            const uint16_t* sc = scales + ((size_t)tl.e * p.l.nb + (n >> 4)) * p.l.groups * 16 + (n & 7) * 2 + ((n >> 3) & 1);
+            const uint16_t* sc = scales + (((size_t)tl.e * p.l.nb + (n >> 4)) * p.l.groups + g0) * 16 + (n & 7) * 2 + ((n >> 3) & 1);
             float sum[H];
 #pragma unroll
             for (int j = 0; j < H; ++j) sum[j] = 0.f;
@@ -382,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
             for (int gi = 0; gi < groups; ++gi, ++ch) {
                 const int u = (int)(ch % NB);
                 const float s = s_next;
-                s_next = there && gi + 1 < p.l.groups ? __uint_as_float((uint32_t)__ldg(sc + (gi + 1) * 16) << 16) : 0.f;
+                s_next = there && g0 + gi + 1 < p.l.groups ? __uint_as_float((uint32_t)__ldg(sc + (gi + 1) * 16) << 16) : 0.f;
                 const bool ready = mbar_wait(&ctl->tmem_full[u], (uint32_t)((ch / NB) & 1), abort, p.err,
                                              kErrTimeoutEpilogue);   // inline: a call would save the sums around it
                 if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
@@ -403,7 +414,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
                 if (lane == 0) mbar_arrive_remote(lead_te0 + (uint32_t)(u * sizeof(uint64_t)));
             }
             if (!ok) break;
-            if (there) {
+            if (p.ks > 1) {                        // the stages are free: this pair's last product is done
+#pragma unroll
+                for (int j = 0; j < H; ++j) red[(half * H + j) * 128 + sp * 32 + lane] = sum[j];
+            } else if (there) {
                 T* c = static_cast<T*>(p.C) + (size_t)(tl.m0 + half * H) * p.ldc + n;
                 const int rows = tl.m1 - tl.m0 - half * H;
 #pragma unroll
@@ -420,6 +434,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc_pair(tmem_base, 512);
+    }
+    if (p.ks > 1) {
+        // every split adds the parts of its share of the tile's rows of A, in the order of the splits
+        if (warp >= 8 && pair < num_tiles) {
+            const Tile tl = tile_of<TN>(p, first, pair);
+            const int row = (warp & 3) * 32 + lane, n = tl.nb * 256 + (int)rank * 128 + row;
+            const int share = H / p.ks, j0 = (int)(crank >> 1) * 2 * share + ((warp - 8) >> 2) * share;
+            for (int j = j0; j < j0 + share; ++j) {
+                if (j >= tl.m1 - tl.m0 || n >= p.N) break;
+                float y = 0.f;
+                for (int q = 0; q < p.ks; ++q) y += ld_shared_cluster(red + j * 128 + row, 2u * q + rank);
+                static_cast<T*>(p.C)[(size_t)(tl.m0 + j) * p.ldc + n] = from_float<T>(y * code_unit<BF16>());
+            }
+        }
+        cluster_sync_all();                        // no CTA leaves while its parts are read
     }
 }
 
@@ -452,6 +481,17 @@ __global__ void __launch_bounds__(256) k_q4_stage(const T* __restrict__ A, long 
     }
 }
 
+long tile_count(const Q4GemmArgs& a, int TN) {
+    return ((a.offsets ? std::min(a.E, a.R) : 0) + ((long)a.R + TN - 1) / TN) * ((a.N + 255) / 256);
+}
+// Few tiles: two or four pairs, in one cluster, share a tile and split its K, each keeping at least 512 values of it
+// (128 x 8192 x 8192 in 32 tiles: 48 -> 34 us with two; 128 x 2048 x 4096 in 8: 25 -> 23 us with two, 15 with four;
+// 128 x 4096 x 4096 in 16: 25 -> 23 with two, but 29 with four, whose clusters of eight CTAs do not all fit at once).
+int k_splits(long tiles, int np, int num_sms) {
+    if (tiles <= 8 && np >= 32) return 4;
+    return tiles * 2 <= num_sms / 2 && np >= 16 ? 2 : 1;
+}
+
 template <typename T, int TN, int GROUP>
 int launch_pair_g(const Q4GemmArgs& a, const void* X, long ldx, int rows, long kx, int plane, cudaStream_t st) {
     constexpr int SL = sizeof(T) == 4 ? 3 : 1;
@@ -482,14 +522,16 @@ int launch_pair_g(const Q4GemmArgs& a, const void* X, long ldx, int rows, long k
     const int e0 = once([&] { return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM); });
     if (e0) return e0;
     // with offsets the number of tiles is known on the device only: at most one partly filled tile per expert
-    const long tiles = ((a.offsets ? std::min(a.E, a.R) : 0) + ((long)a.R + TN - 1) / TN) * p.num_n;
+    const long tiles = tile_count(a, TN);
+    p.ks = TN <= 128 ? k_splits(tiles, p.np, a.num_sms) : 1;
+    p.span = (p.np / 2 + p.ks - 1) / p.ks * 2;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.x = 2 * p.ks;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(2 * std::min((long)a.num_sms / 2, tiles)), 1, 1);
+    cfg.gridDim = dim3((unsigned)(2 * p.ks * (p.ks > 1 ? tiles : std::min((long)a.num_sms / 2, tiles))), 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = C_::SMEM;
     cfg.stream = st;
@@ -528,8 +570,13 @@ int launch_t(const Q4GemmArgs& a, cudaStream_t st) {
         if (e != cudaSuccess) return (int)e;
         X = a.stage;
     }
-    const long each = a.R / std::max(1, a.offsets ? std::min(a.E, a.R) : 1);
-    if (each > 128) return launch_pair<T, 256>(a, X, ldx, rows, kx, plane, st);
+    // 256 or 128 rows of A per tile, whichever is done sooner: rounds of the pairs times a panel's time, 1.3 times as long
+    // for 256 (0.49 against 0.375 us at 8192 x 8192).
+    const int pairs = a.num_sms / 2, np = (int)((a.K + 127) / 128 * 2);
+    const long t128 = tile_count(a, 128), t256 = tile_count(a, 256);
+    const int ks = k_splits(t128, np, a.num_sms);
+    const double c128 = (double)((t128 * ks + pairs - 1) / pairs) / ks, c256 = 1.3 * (double)((t256 + pairs - 1) / pairs);
+    if (c256 <= c128) return launch_pair<T, 256>(a, X, ldx, rows, kx, plane, st);
     return launch_pair<T, 128>(a, X, ldx, rows, kx, plane, st);
 }
 

@@ -44,7 +44,10 @@ emugemm_status_t q4_product(emugemm_handle_t handle, int R, int E, int N, long K
     a.err = h->err_dev;
     const int with = experts ? (E < R ? E : R) : 1;   // experts that can have rows
     const long cols = (long)(R / with) * (dtype == EMU_DTYPE_F32 ? 3 : 1);
-    if (cols <= 48) {
+    // Few columns: one pass over the codes per 48 of them (k_q4.cu), else tiles of CTA pairs (k_q4_tc.cu). 8192 x 8192,
+    // groups of 128: 48 columns 37 against 34 us, 64 (two passes) 64 against 34; 4096 x 4096: 14 against 23 and 23 against
+    // 23. Groups of 32 cost the tiles an accumulator each, the passes nothing: 64 columns 27 against 41 us.
+    if (cols <= (group == 32 ? 96 : 48)) {
         ProfScope ps(h, kProfQ4);
         return from_cuda(launch_q4_rows(a, h->stream));
     }

@@ -288,8 +288,12 @@ void emugemm_test_stall_next_launches(int n);
    experts with weights of their own and back. All matrices are row-major device buffers of the handle's device; A, C
    and the routed rows are FP32, FP16 or BF16 (emu_dtype_t, the same type in and out), every leading dimension counts
    elements and may exceed the row length, inputs and outputs must not overlap. The calls are asynchronous on the
-   handle's stream, allocate nothing and can be captured into CUDA graphs. Sums are FP32 in a fixed order (no atomics):
-   the same call gives the same bits. Status: INVALID_VALUE for an unknown dtype or group, INVALID_SIZE for a size or
+   handle's stream and can be captured into CUDA graphs. Only products of many rows use the handle's workspace, for rows of
+   A that a tile load cannot read in place (FP32, or 16-bit rows not on 16-byte boundaries): such a call returns
+   MEMORY_ERROR while capturing unless one of its size ran before, what a captured graph uses stays until the handle is
+   destroyed, and calls and replays of one handle must be ordered on the GPU, as all its calls. Sums are FP32 in a fixed
+   order (no atomics): the same call gives the same bits. A device-side wait that gave up is reported by emugemm_sync
+   (TIMEOUT). Status: INVALID_VALUE for an unknown dtype or group, INVALID_SIZE for a size or
    leading dimension out of range, INVALID_POINTER for a null or misaligned pointer (elements by their size, packed
    weights by 16 bytes). Device-side indices (offsets, place) are bounds-checked by the kernels: a bad one touches no
    memory outside the given matrices. */

@@ -154,6 +154,20 @@ def test_product(cuda, handle, kind, M, N, K, group):
     check_product(cuda, handle, M, N, K, group, kind)
 
 
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("M,N,K,group", [(100, 300, 2200, 64), (70, 600, 4100, 128), (128, 4096, 1100, 32), (90, 2500, 1024, 64),
+                                         (60, 256, 6500, 32), (127, 4100, 2176, 128)])
+def test_product_k_splits(cuda, handle, kind, M, N, K, group):
+    """Few tiles: two or four CTA pairs share a tile and split its K, also into parts that are not equal."""
+    check_product(cuda, handle, M, N, K, group, kind)
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("counts", [[60, 70, 0, 90], [0, 130, 1], [55] * 6])
+def test_experts_k_splits(cuda, handle, kind, counts):
+    check_experts(cuda, handle, counts, 200, 2100, 32, kind, tail=5)
+
+
 @pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
 @pytest.mark.parametrize("M", [1, 6, 40, 150])
 @pytest.mark.parametrize("lda,ldc", [(200, 96), (201, 97), (208, 104)])
@@ -358,6 +372,48 @@ def test_capture_and_replay_with_new_inputs(cuda, M, kind):
             assert torch.equal(c, want)
         h.sync()
         del graph
+
+
+def test_capture_needs_the_workspace_first(cuda):
+    """Many FP32 rows are staged in the workspace: captured on a handle that never ran the size, the call is refused, the
+    capture stays valid and the handle usable."""
+    torch = cuda
+    M, N, K, group = 300, 64, 256, 64
+    packed, w = q4ref.weights(5, 1, N, K, group)
+    a, c = torch.randn(M, K, generator=torch.Generator().manual_seed(1)).cuda(), torch.zeros(M, N, device="cuda")
+    st = torch.cuda.Stream()
+    with emugemm.Handle(st) as h, torch.cuda.stream(st):
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            with pytest.raises(emugemm.EmuGemmError) as e:
+                h.q4_gemm(M, N, K, a, K, packed, group, c, N)
+            assert e.value.code == 5        # MEMORY_ERROR
+            c.add_(1)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (c == 1).all()
+        h.q4_gemm(M, N, K, a, K, packed, group, c, N)
+        h.sync()
+        xd = a.double().cpu().numpy()
+        ref = xd @ w[0].T
+        assert (np.abs(c.double().cpu().numpy() - ref) <= q4ref.product_bound(xd, w[0], ref, group, "fp32")).all()
+        del graph
+
+
+def test_workspace_limit(cuda):
+    torch = cuda
+    packed, _ = q4ref.weights(5, 1, 32, 64, 32)
+    a, c = torch.ones(200, 64, device="cuda"), torch.empty(200, 32, device="cuda")
+    with emugemm.Handle() as h:
+        h.set_workspace_limit(1024)
+        with pytest.raises(emugemm.EmuGemmError) as e:
+            h.q4_gemm(200, 32, 64, a, 64, packed, 32, c, 32)
+        assert e.value.code == 5
+        h.q4_gemm(2, 32, 64, a, 64, packed, 32, c, 32)     # few rows need none
+        h.set_workspace_limit(0)
+        h.q4_gemm(200, 32, 64, a, 64, packed, 32, c, 32)
+        h.sync()
 
 
 def test_two_handles_on_two_streams(cuda):
