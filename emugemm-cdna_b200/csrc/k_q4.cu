@@ -403,7 +403,6 @@ __device__ __forceinline__ void stage_rows(uint16_t* xs, int pitch, const T* row
     while (true) {
         while (k0 >= span) {
             k0 -= (span + 255) / 256 * 256;
-            if (k0 < 0) k0 = 0;
             if (++m >= toks) return;
         }
         const T* row = rows + (size_t)m * lda;
@@ -593,13 +592,31 @@ __global__ void __launch_bounds__(32 * kWarps, CTAS) k_q4_rows(RowsParams p) {
             const long n = rb0 * 16 + row;
             float y = 0.f;
 #pragma unroll
-            for (int s = SL - 1; s >= 0; --s)
-                for (uint32_t c = 0; c < csize; ++c)
+            for (int s = SL - 1; s >= 0; --s) {
+                const float* q = red + (m * SL + s) * ROWS + row;
+                if (csize == 1) {
+#pragma unroll
+                    for (int k = 0; k < WK; ++k) y += q[k * COLS * ROWS];
+                } else if (WK >= 4) {                // the parts of a CTA, or of the cluster, on their way together
+                    for (uint32_t c = 0; c < csize; ++c) {
+                        float v[WK];
+#pragma unroll
+                        for (int k = 0; k < WK; ++k) v[k] = ld_cluster(q + k * COLS * ROWS, c);
+#pragma unroll
+                        for (int k = 0; k < WK; ++k) y += v[k];
+                    }
+                } else {
 #pragma unroll
                     for (int k = 0; k < WK; ++k) {
-                        const float* q = red + (k * COLS + m * SL + s) * ROWS + row;
-                        y += csize > 1 ? ld_cluster(q, c) : *q;
+                        float v[8];
+#pragma unroll
+                        for (uint32_t c = 0; c < 8; ++c) v[c] = c < csize ? ld_cluster(q + k * COLS * ROWS, c) : 0.f;
+#pragma unroll
+                        for (uint32_t c = 0; c < 8; ++c)
+                            if (c < csize) y += v[c];
                     }
+                }
+            }
             if (n < p.N) static_cast<T*>(p.C)[(size_t)(c0 + m) * p.ldc + n] = from_float<T>(y * code_unit<BF16>());
         }
         // the next pass, or the exit, waits for the others' reads
@@ -614,7 +631,8 @@ int launch_rows_g(RowsParams p, int num_sms, cudaStream_t st) {
     constexpr int STEP = kWarps / WR * D * 128;                // values of K that the warps hold in flight
     const long groups = (p.l.nb + WR * RBW - 1) / (WR * RBW);
     const int experts = p.offsets ? std::min(p.E, p.R) : 1;
-    // K split over a cluster while all CTAs are resident at once and each keeps a step of its warps
+    // K split over a cluster while all CTAs are resident at once and each keeps a step of its warps; single rows only below
+    // one CTA per SM (a cluster of two takes about 2 us longer to launch than its CTAs alone)
     int ck = 1;
     while (ck < 8 && groups * experts * ck * 2 <= (long)(NT == 1 && WR == 1 ? 1 : CTAS) * num_sms && p.K >= 2L * ck * STEP) ck *= 2;
     p.kspan = (int)(((p.K + ck - 1) / ck + 127) / 128 * 128);
