@@ -11,6 +11,7 @@ import ctypes
 import os
 import pathlib
 import re
+import sys
 
 HERE = pathlib.Path(__file__).resolve().parent
 LIB_PATH = HERE / "libemugemm.so"
@@ -203,19 +204,6 @@ def _dtype(dtype, *xs) -> int:
     return dtype
 
 
-def _typed(x, name: str) -> int:
-    """Pointer of x, which, if a tensor, must have the dtype `name` (ValueError)."""
-    d = getattr(x, "dtype", None)
-    if d is None:
-        return _ptr(x)
-    known = _dtype_names.get(d)
-    if known is None:
-        known = _dtype_names[d] = str(d)
-    if known != name:
-        raise ValueError(f"expected a {name} tensor, got {d}")
-    return x.data_ptr()
-
-
 def q4_bytes(E: int, N: int, K: int, group: int) -> int:
     """Bytes of the packed 4-bit weights of E experts of N x K (emugemm_q4_bytes); 0 when a size is out of range."""
     return int(lib().emugemm_q4_bytes(E, N, K, group))
@@ -249,6 +237,8 @@ class Handle:
         h = c_void_p()
         check("emugemm_create_handle", lib().emugemm_create_handle(ctypes.byref(h)))
         self.h = h
+        torch = sys.modules.get("torch")
+        self.device = torch.cuda.current_device() if torch is not None else None   # of the tensors it may be given
         if stream is not None:
             self.set_stream(stream)
         # kernel choices as created (from the environment), restored by reset_kernels()
@@ -413,59 +403,75 @@ class Handle:
     def split_f16(self, X, n, hi, lo) -> None:
         check("emugemm_split_f16", lib().emugemm_split_f16(self.h, _ptr(X), n, _ptr(hi), _ptr(lo)))
 
+    def _at(self, x, name: str | None = None) -> int:
+        """Address of x (None, an address, or a tensor). A tensor must be on the handle's device and, with `name`, have that
+        dtype (ValueError): a kernel given a host address or another type's bytes would fault or compute nonsense."""
+        if x is None or isinstance(x, int):
+            return x or 0
+        if self.device is not None and x.get_device() != self.device:
+            raise ValueError(f"expected a tensor on cuda:{self.device}, got one on {x.device}")
+        if name is not None:
+            d = x.dtype
+            known = _dtype_names.get(d)
+            if known is None:
+                known = _dtype_names[d] = str(d)
+            if known != name:
+                raise ValueError(f"expected a {name} tensor, got {d}")
+        return x.data_ptr()
+
     # ---- 4-bit weights and expert routing (dtype: from the tensors, or emugemm.F32 / F16 / BF16 for raw pointers) ----
     def q4_pack(self, E, N, K, W, ldw, group, packed, dtype=None) -> None:
         """Quantise E * N rows of K weights into `packed` (q4_bytes(E, N, K, group) bytes)."""
-        check("emugemm_q4_pack", lib().emugemm_q4_pack(self.h, E, N, K, _ptr(W), ldw, _dtype(dtype, W), group,
-                                                       _ptr(packed)))
+        check("emugemm_q4_pack", lib().emugemm_q4_pack(self.h, E, N, K, self._at(W), ldw, _dtype(dtype, W), group,
+                                                       self._at(packed)))
 
     def q4_unpack(self, E, N, K, group, packed, W, ldw) -> None:
         """The FP32 values of packed weights."""
-        check("emugemm_q4_unpack", lib().emugemm_q4_unpack(self.h, E, N, K, group, _ptr(packed),
-                                                           _typed(W, "torch.float32"), ldw))
+        check("emugemm_q4_unpack", lib().emugemm_q4_unpack(self.h, E, N, K, group, self._at(packed),
+                                                           self._at(W, "torch.float32"), ldw))
 
     def q4_gemm(self, M, N, K, A, lda, packed, group, C, ldc, dtype=None) -> None:
         """C (M x N) = A (M x K) * W^T with packed 4-bit weights."""
-        check("emugemm_q4_gemm", lib().emugemm_q4_gemm(self.h, M, N, K, _ptr(A), lda, _dtype(dtype, A, C), _ptr(packed),
-                                                       group, _ptr(C), ldc))
+        check("emugemm_q4_gemm", lib().emugemm_q4_gemm(self.h, M, N, K, self._at(A), lda, _dtype(dtype, A, C), self._at(packed),
+                                                       group, self._at(C), ldc))
 
     def q4_gemm_experts(self, R, E, N, K, A, lda, offsets, packed, group, C, ldc, dtype=None) -> None:
         """q4_gemm with weights of E experts over rows sorted by expert (offsets: E + 1 int32 on the device)."""
         check("emugemm_q4_gemm_experts",
-              lib().emugemm_q4_gemm_experts(self.h, R, E, N, K, _ptr(A), lda, _dtype(dtype, A, C),
-                                            _typed(offsets, "torch.int32"), _ptr(packed), group, _ptr(C), ldc))
+              lib().emugemm_q4_gemm_experts(self.h, R, E, N, K, self._at(A), lda, _dtype(dtype, A, C),
+                                            self._at(offsets, "torch.int32"), self._at(packed), group, self._at(C), ldc))
 
     def expert_sort(self, T, topk, E, expert, order, place, offsets) -> None:
         """Stable sort of T x topk expert ids; all arrays int32."""
         i = "torch.int32"
-        check("emugemm_expert_sort", lib().emugemm_expert_sort(self.h, T, topk, E, _typed(expert, i), _typed(order, i),
-                                                               _typed(place, i), _typed(offsets, i)))
+        check("emugemm_expert_sort", lib().emugemm_expert_sort(self.h, T, topk, E, self._at(expert, i), self._at(order, i),
+                                                               self._at(place, i), self._at(offsets, i)))
 
     def expert_gather(self, T, topk, H, X, ldx, place, XS, ldxs, dtype=None) -> None:
         """XS[place[t, j]] = X[t]."""
-        check("emugemm_expert_gather", lib().emugemm_expert_gather(self.h, T, topk, H, _ptr(X), ldx, _dtype(dtype, X, XS),
-                                                                   _typed(place, "torch.int32"), _ptr(XS), ldxs))
+        check("emugemm_expert_gather", lib().emugemm_expert_gather(self.h, T, topk, H, self._at(X), ldx, _dtype(dtype, X, XS),
+                                                                   self._at(place, "torch.int32"), self._at(XS), ldxs))
 
     def expert_gather_backward(self, T, topk, H, dXS, lddxs, place, dX, lddx, dtype=None) -> None:
         """dX[t] = sum over j of dXS[place[t, j]]."""
         check("emugemm_expert_gather_backward",
-              lib().emugemm_expert_gather_backward(self.h, T, topk, H, _ptr(dXS), lddxs, _dtype(dtype, dXS, dX),
-                                                   _typed(place, "torch.int32"), _ptr(dX), lddx))
+              lib().emugemm_expert_gather_backward(self.h, T, topk, H, self._at(dXS), lddxs, _dtype(dtype, dXS, dX),
+                                                   self._at(place, "torch.int32"), self._at(dX), lddx))
 
     def expert_combine(self, T, topk, H, YS, ldys, place, weights, Y, ldy, dtype=None) -> None:
         """Y[t] = sum over j of weights[t, j] * YS[place[t, j]] (weights float32)."""
         check("emugemm_expert_combine",
-              lib().emugemm_expert_combine(self.h, T, topk, H, _ptr(YS), ldys, _dtype(dtype, YS, Y),
-                                           _typed(place, "torch.int32"), _typed(weights, "torch.float32"), _ptr(Y), ldy))
+              lib().emugemm_expert_combine(self.h, T, topk, H, self._at(YS), ldys, _dtype(dtype, YS, Y),
+                                           self._at(place, "torch.int32"), self._at(weights, "torch.float32"), self._at(Y), ldy))
 
     def expert_combine_backward(self, T, topk, H, dY, lddy, YS, ldys, place, weights, dYS, lddys, dweights,
                                 dtype=None) -> None:
         """dYS[place[t, j]] = weights[t, j] * dY[t] and dweights[t, j] = <dY[t], YS[place[t, j]]>."""
         f = "torch.float32"
         check("emugemm_expert_combine_backward",
-              lib().emugemm_expert_combine_backward(self.h, T, topk, H, _ptr(dY), lddy, _ptr(YS), ldys,
-                                                    _dtype(dtype, dY, YS, dYS), _typed(place, "torch.int32"),
-                                                    _typed(weights, f), _ptr(dYS), lddys, _typed(dweights, f)))
+              lib().emugemm_expert_combine_backward(self.h, T, topk, H, self._at(dY), lddy, self._at(YS), ldys,
+                                                    _dtype(dtype, dY, YS, dYS), self._at(place, "torch.int32"),
+                                                    self._at(weights, f), self._at(dYS), lddys, self._at(dweights, f)))
 
     PROF_KINDS = ["tc_gemm", "fp32_gemm", "split", "scan", "rho", "reduce", "q4", "expert"]
 

@@ -333,7 +333,8 @@ emugemm_status_t emugemm_q4_gemm_experts(emugemm_handle_t handle, int R, int E, 
    id outside [0, E) (a dropped or padding token) has no row: place[s] = -1, and order is -1 from offsets[E] on. */
 emugemm_status_t emugemm_expert_sort(emugemm_handle_t handle, int T, int topk, int E, const int* expert, int* order,
                                      int* place, int* offsets);
-/* XS[place[t, j]] = X[t] (rows of H). Rows of XS that no slot has are left as they were. */
+/* XS[place[t, j]] = X[t] (rows of H; XS, as every sorted matrix of these calls, has room for T * topk rows). Rows of XS that
+   no slot has are left as they were. */
 emugemm_status_t emugemm_expert_gather(emugemm_handle_t handle, int T, int topk, int H, const void* X, long ldx, int dtype,
                                        const int* place, void* XS, long ldxs);
 /* Gradient of emugemm_expert_gather: dX[t] = sum over j of dXS[place[t, j]]; 0 for a token without an expert. */

@@ -159,8 +159,15 @@ def test_binding_checks_tensor_types():
         emugemm._dtype(emugemm.F16, x)
     with pytest.raises(ValueError):
         emugemm._dtype(None, 4096)
+    h = emugemm.Handle.__new__(emugemm.Handle)      # the checks need no device
+    h.h, h.device = None, -1                        # -1: the host, where these tensors are
+    i = torch.zeros(4, dtype=torch.int32)
+    assert h._at(i, "torch.int32") == i.data_ptr() and h._at(None) == 0 and h._at(4096, "torch.int32") == 4096
     with pytest.raises(ValueError):
-        emugemm._typed(torch.zeros(4, dtype=torch.int64), "torch.int32")
+        h._at(torch.zeros(4, dtype=torch.int64), "torch.int32")
+    h.device = 0
+    with pytest.raises(ValueError):
+        h._at(i, "torch.int32")                     # a host tensor
 
 
 def test_every_entry_point_is_bound():
