@@ -76,6 +76,7 @@ struct Params {
     int num_n;                      // 256-row tiles of the weights
     int np;                         // panels per tile (even)
     int ks, span;                   // K splits (pairs per cluster), panels of each (even; the last may have fewer)
+    int wide;                       // 16-bit C that 16-byte stores of 8 columns fit
     int plane;                      // rows between the slices of A (SL = 3)
     unsigned* err;
 };
@@ -123,6 +124,46 @@ __device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
                    "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                  :
                  : "memory");
+}
+
+// 32 lanes' columns of H rows of C (y[j]: row j, this lane's column) as 16-byte stores: three rounds of exchanges between
+// lanes 1, 2 and 4 apart turn pairs of rows into pairs of columns, so that lane l ends with columns 8 (l >> 3) .. + 7 of row
+// 8 q + (l & 7) for each q. (2-byte stores, 64 contiguous bytes a warp, took about 80 cycles each: 28 % of 16384 rows over 16
+// experts, 4096 x 2048.) c: row 0, the warp's first column.
+template <typename T, int H>
+__device__ __forceinline__ void store_wide(T* c, long ldc, int rows, int cols, const float (&y)[H], float unit) {
+    const int lane = threadIdx.x & 31;
+    const bool o1 = lane & 1, o2 = lane & 2, o3 = lane & 4;
+    uint32_t w[H / 2];
+#pragma unroll
+    for (int i = 0; i < H / 2; ++i) {
+        const float a = y[2 * i] * unit, b = y[2 * i + 1] * unit;
+        if (std::is_same<T, __half>::value) {
+            const __half2 h = __floats2half2_rn(a, b);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, w[i], 1);
+        w[i] = __byte_perm(w[i], other, o1 ? 0x3276 : 0x5410);
+    }
+#pragma unroll
+    for (int q = 0; q < H / 4; ++q) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, o2 ? w[2 * q] : w[2 * q + 1], 2);
+        if (o2) w[2 * q] = other;
+        else w[2 * q + 1] = other;
+    }
+    T* to = c + (size_t)(lane & 7) * ldc + 8 * (lane >> 3);
+    const bool in = 8 * (lane >> 3) < cols;
+#pragma unroll
+    for (int q = 0; q < H / 8; ++q) {
+        const uint32_t r0 = __shfl_xor_sync(0xffffffffu, o3 ? w[4 * q] : w[4 * q + 2], 4);
+        const uint32_t r1 = __shfl_xor_sync(0xffffffffu, o3 ? w[4 * q + 1] : w[4 * q + 3], 4);
+        const uint4 v = o3 ? make_uint4(r0, r1, w[4 * q + 2], w[4 * q + 3]) : make_uint4(w[4 * q], w[4 * q + 1], r0, r1);
+        if (in && 8 * q + (lane & 7) < rows) *reinterpret_cast<uint4*>(to) = v;
+        to += 8 * ldc;
+    }
 }
 
 // The tile's expert, 256-row block of weights, and rows [m0, m1) of A. first[e] is the first row tile of expert e.
@@ -417,6 +458,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
             if (p.ks > 1) {                        // the stages are free: this pair's last product is done
 #pragma unroll
                 for (int j = 0; j < H; ++j) red[(half * H + j) * 128 + sp * 32 + lane] = sum[j];
+            } else if (SL == 1 && p.wide) {
+                const int n0 = n - lane;
+                store_wide<T, H>(static_cast<T*>(p.C) + (size_t)(tl.m0 + half * H) * p.ldc + n0, p.ldc,
+                                 tl.m1 - tl.m0 - half * H, p.N - n0, sum, code_unit<BF16>());
             } else if (there) {
                 T* c = static_cast<T*>(p.C) + (size_t)(tl.m0 + half * H) * p.ldc + n;
                 const int rows = tl.m1 - tl.m0 - half * H;
@@ -516,6 +561,7 @@ int launch_pair_g(const Q4GemmArgs& a, const void* X, long ldx, int rows, long k
     p.num_n = (a.N + 255) / 256;
     p.np = (int)((a.K + 127) / 128 * 2);
     p.plane = plane;
+    p.wide = SL == 1 && (reinterpret_cast<uintptr_t>(a.C) & 15) == 0 && a.ldc % 8 == 0 && a.N % 8 == 0;
     p.err = a.err;
     auto kern = k_q4_pair<T, TN, GROUP>;
     static OncePerDevice once;
