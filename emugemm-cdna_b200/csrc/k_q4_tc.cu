@@ -486,11 +486,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
             const Tile tl = tile_of<TN>(p, first, pair);
             const int row = (warp & 3) * 32 + lane, n = tl.nb * 256 + (int)rank * 128 + row;
             const int share = H / p.ks, j0 = (int)(crank >> 1) * 2 * share + ((warp - 8) >> 2) * share;
-            for (int j = j0; j < j0 + share; ++j) {
-                if (j >= tl.m1 - tl.m0 || n >= p.N) break;
-                float y = 0.f;
-                for (int q = 0; q < p.ks; ++q) y += ld_shared_cluster(red + j * 128 + row, 2u * q + rank);
-                static_cast<T*>(p.C)[(size_t)(tl.m0 + j) * p.ldc + n] = from_float<T>(y * code_unit<BF16>());
+            const int j1 = n < p.N ? min(j0 + share, tl.m1 - tl.m0) : j0;
+            T* c = static_cast<T*>(p.C) + (size_t)tl.m0 * p.ldc + n;
+            for (int j = j0; j < j1; j += 4) {       // the parts of four rows of A on their way together
+                float v[4][4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        v[q][i] = q < p.ks && j + i < j1 ? ld_shared_cluster(red + (j + i) * 128 + row, 2u * q + rank) : 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (j + i < j1)
+                        c[(size_t)(j + i) * p.ldc] = from_float<T>((v[0][i] + v[1][i] + v[2][i] + v[3][i]) * code_unit<BF16>());
             }
         }
         cluster_sync_all();                        // no CTA leaves while its parts are read
