@@ -234,19 +234,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
         tmem_relinquish_pair();
     }
     if (warp == 2 && p.offsets) {
+        // offsets that run backwards or overlap make no more tiles than the host counted for (tile_count)
+        const int cap = min(p.E, p.R) + (p.R + TN - 1) / TN;
         int run = 0;
         for (int x0 = 0; x0 < p.E; x0 += 32) {
             const int x = x0 + lane;
-            const int rows = x < p.E ? min(p.R, p.offsets[x + 1]) - max(0, p.offsets[x]) : 0;
-            const int n = rows > 0 ? (rows + TN - 1) / TN : 0;
+            const int r0 = x < p.E ? max(0, p.offsets[x]) : 0, r1 = x < p.E ? min(p.R, p.offsets[x + 1]) : 0;
+            const int n = r1 > r0 ? (r1 - r0 + TN - 1) / TN : 0;
             int inc = n;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
                 const int v = __shfl_up_sync(0xffffffffu, inc, d);
                 if (lane >= d) inc += v;
             }
-            if (x < p.E) first[x] = run + inc - n;
-            run += __shfl_sync(0xffffffffu, inc, 31);
+            if (x < p.E) first[x] = min(run + inc - n, cap);
+            run = min(run + __shfl_sync(0xffffffffu, inc, 31), cap);
         }
         if (lane == 0) first[p.E] = run;
     }
@@ -254,8 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = ctl->tmem_base;
-    int num_tiles = (p.offsets ? first[p.E] : (p.R + TN - 1) / TN) * p.num_n;
-    if (p.ks > 1) num_tiles = min(num_tiles, num_pairs);   // one tile per cluster (more only with overlapping offsets)
+    const int num_tiles = (p.offsets ? first[p.E] : (p.R + TN - 1) / TN) * p.num_n;   // ks > 1: at most one per cluster
 
     if (warp < 8) {
         reg_dec<kRegOther>();

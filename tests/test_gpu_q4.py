@@ -339,6 +339,26 @@ def test_experts_bad_offsets_stay_inside(cuda, handle, R):
         assert not c[R:2 * R].isnan().any()
 
 
+@pytest.mark.parametrize("N,K", [(32, 128), (264, 2048)])
+def test_experts_extreme_offsets_stay_inside(cuda, handle, N, K):
+    """Offsets at the ends of int32, whose differences wrap, and all rows claimed by every expert: nothing outside of C is
+    written, and the next call of the handle is right."""
+    torch = cuda
+    lo, hi = -2 ** 31, 2 ** 31 - 1
+    E, R, group = 5, 400, 64
+    packed, w = q4ref.weights(1, E, N, K, group)
+    a = torch.full((3 * R, K), float("nan"), dtype=torch.bfloat16, device="cuda")
+    a[R:2 * R] = 1
+    c = torch.full((3 * R, N), -7.5, dtype=torch.bfloat16, device="cuda")
+    for off in ([hi, lo, hi, lo, hi, lo], [lo, hi, lo, hi, lo, hi], [0, R, 0, R, 0, R], [hi] * 6, [lo] * 6):
+        handle.q4_gemm_experts(R, E, N, K, a[R:], K, torch.tensor(off, dtype=torch.int32, device="cuda"), packed, group,
+                               c[R:], N)
+        handle.sync()
+        assert (c[:R] == -7.5).all() and (c[2 * R:] == -7.5).all()
+        assert not c[R:2 * R].isnan().any()
+    check_experts(torch, handle, [80] * 5, N, K, group, "bf16")
+
+
 # -------------------------------------------------------------------------------- streams, graphs, handles, workspace
 @pytest.mark.parametrize("M,kind", [(1, "bf16"), (40, "fp32"), (200, "fp32"), (200, "bf16")])
 def test_capture_and_replay_with_new_inputs(cuda, M, kind):
