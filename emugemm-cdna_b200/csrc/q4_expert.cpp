@@ -16,9 +16,10 @@ bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
 // a pointer the kernels may access with its element's (or the packed layout's) alignment
 bool bad_ptr(const void* p, int align) { return !p || (reinterpret_cast<uintptr_t>(p) & (align - 1)); }
 
-// Sizes of packed weights: E experts of N x K (K below 2^31, all code bytes addressable)
+// Sizes of packed weights: E experts of N x K, of which no count of bytes or tiles passes 63 bits
 bool q4_size_ok(int E, int N, long K) {
-    return E >= 1 && E <= kMaxExperts && N >= 1 && N <= (1 << 30) && K >= 1 && K <= (1L << 30);
+    return E >= 1 && E <= kMaxExperts && N >= 1 && N <= (1 << 30) && K >= 1 && K <= (1L << 30) &&
+           (long)E * N <= (1L << 50) / K;
 }
 // Sizes of the routing calls: at most 2^30 slots
 bool slots_ok(long T, int topk) { return T >= 0 && topk >= 1 && (T == 0 || topk <= (1L << 30) / T); }

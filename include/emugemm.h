@@ -300,8 +300,9 @@ void emugemm_test_stall_next_launches(int n);
 typedef enum { EMU_DTYPE_F32 = 0, EMU_DTYPE_F16 = 1, EMU_DTYPE_BF16 = 2 } emu_dtype_t;
 
 /* Bytes of the packed weights of E experts (1 for a plain matrix; at most 1024) of N x K, with one scale per `group`
-   (32, 64 or 128) values along K; the last group of a row may be shorter. 0 when a size is out of range. Layout (a
-   program may also write it itself, from weights quantised elsewhere to q = -8..7 and bf16 scales):
+   (32, 64 or 128) values along K; the last group of a row may be shorter. 0 when a size is out of range (at most 2^30
+   rows, 2^30 values of K and 2^50 weights in all). Layout (a program may also write it itself, from weights quantised
+   elsewhere to q = -8..7 and bf16 scales):
      codes: q + 8 (8 = zero in the padding), N padded to 16 rows and K to 64; tiles of 16 rows x 64 values of K of 512
        bytes, ordered [expert][row block][k block]; bytes (4g + t) * 16 .. + 15 of a tile (g = 0..7, t = 0..3) are four
        32-bit words: row g at k = 8t..8t+7, row g + 8 at the same k, row g at k = 32 + 8t.., row g + 8 at the same; in a

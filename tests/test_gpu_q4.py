@@ -162,6 +162,14 @@ def test_product_k_splits(cuda, handle, kind, M, N, K, group):
     check_product(cuda, handle, M, N, K, group, kind)
 
 
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("M,N,K,group", [(300, 8, 128, 32), (150, 104, 200, 64), (1000, 2008, 256, 128), (777, 1288, 65, 128)])
+def test_product_wide_stores(cuda, handle, kind, M, N, K, group):
+    """Columns in eights that end inside a warp's 32 and a CTA's 128, rows inside a tile."""
+    check_product(cuda, handle, M, N, K, group, kind)
+    check_product(cuda, handle, M, N, K, group, kind, ldc=N + 24)
+
+
 @pytest.mark.parametrize("kind", ["fp32", "bf16"])
 @pytest.mark.parametrize("counts", [[60, 70, 0, 90], [0, 130, 1], [55] * 6])
 def test_experts_k_splits(cuda, handle, kind, counts):

@@ -34,6 +34,13 @@ def test_q4_bytes_out_of_range(E, N, K, group):
     assert emugemm.q4_bytes(E, N, K, group) == 0
 
 
+@pytest.mark.parametrize("E,N,K", [(1024, 1 << 30, 1 << 30), (1024, 1 << 20, (1 << 20) + 1), (1, 1 << 30, 1 << 30)])
+def test_q4_bytes_of_more_than_memory(E, N, K):
+    """More than 2^50 weights: the count of bytes would wrap, so they are refused."""
+    assert emugemm.q4_bytes(E, N, K, 32) == 0
+    assert emugemm.q4_bytes(1024, 1 << 20, 1 << 20, 32) == 2 ** 49 + 2 ** 46
+
+
 def test_layout_restatement_round_trip():
     """q4ref.pack against the layout read back nibble by nibble."""
     E, N, K, group = 2, 19, 70, 32
