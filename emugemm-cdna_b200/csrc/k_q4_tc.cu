@@ -75,7 +75,7 @@ struct Params {
     int R, E, N;
     int num_n;                      // 256-row tiles of the weights
     int np;                         // panels per tile (even)
-    int ks, span;                   // K splits (pairs per cluster), panels of each (even; the last may have fewer)
+    int ks, span;                   // K splits (pairs per cluster, at most 4), panels of each (even; the last may have fewer)
     int wide;                       // 16-bit C that 16-byte stores of 8 columns fit
     int plane;                      // rows between the slices of A (SL = 3)
     unsigned* err;
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
         if (warp >= 8 && pair < num_tiles) {
             const Tile tl = tile_of<TN>(p, first, pair);
             const int row = (warp & 3) * 32 + lane, n = tl.nb * 256 + (int)rank * 128 + row;
-            const int share = H / p.ks, j0 = (int)(crank >> 1) * 2 * share + ((warp - 8) >> 2) * share;
+            const int share = (H + p.ks - 1) / p.ks, j0 = (int)(crank >> 1) * 2 * share + ((warp - 8) >> 2) * share;
             const int j1 = n < p.N ? min(j0 + share, tl.m1 - tl.m0) : j0;
             T* c = static_cast<T*>(p.C) + (size_t)tl.m0 * p.ldc + n;
             for (int j = j0; j < j1; j += 4) {       // the parts of four rows of A on their way together
@@ -538,16 +538,54 @@ __global__ void __launch_bounds__(256) k_q4_stage(const T* __restrict__ A, long 
 long tile_count(const Q4GemmArgs& a, int TN) {
     return ((a.offsets ? std::min(a.E, a.R) : 0) + ((long)a.R + TN - 1) / TN) * ((a.N + 255) / 256);
 }
-// Few tiles: two or four pairs, in one cluster, share a tile and split its K, each keeping at least 512 values of it
-// (128 x 8192 x 8192 in 32 tiles: 48 -> 34 us with two; 128 x 2048 x 4096 in 8: 25 -> 23 us with two, 15 with four;
-// 128 x 4096 x 4096 in 16: 25 -> 23 with two, but 29 with four, whose clusters of eight CTAs do not all fit at once).
-int k_splits(long tiles, int np, int num_sms) {
-    if (tiles <= 8 && np >= 32) return 4;
-    return tiles * 2 <= num_sms / 2 && np >= 16 ? 2 : 1;
+// How many clusters of 2, 3 and 4 pairs the device holds at once (a pair keeps two SMs; SMs left over in a GPC hold none).
+struct Fits { int of[5]; };
+template <typename T>
+int cluster_fits(Fits& f) {
+    static std::atomic<unsigned> known[64];          // 10 bits each, per device
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    unsigned k = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0u;
+    if (!k) {
+        auto kern = k_q4_pair<T, 128, 128>;          // the others take as many threads and (nearly) as much shared memory
+        constexpr int smem = Cfg<sizeof(T) == 4 ? 3 : 1, 128>::SMEM;
+        const cudaError_t a = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (a != cudaSuccess) return (int)a;
+        for (int ks = 2; ks <= 4; ++ks) {
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 2 * ks;
+            attr[0].val.clusterDim.y = 1;
+            attr[0].val.clusterDim.z = 1;
+            cfg.gridDim = dim3(2 * ks, 1, 1);
+            cfg.blockDim = dim3(kThreads, 1, 1);
+            cfg.dynamicSmemBytes = smem;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int n = 0;
+            const cudaError_t o = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+            if (o != cudaSuccess) return (int)o;
+            k |= (unsigned)std::min(n, 1023) << (10 * (ks - 2));
+        }
+        if (dev < 64) known[dev].store(k | 1u << 30, std::memory_order_relaxed);
+    }
+    for (int ks = 2; ks <= 4; ++ks) f.of[ks] = (int)(k >> (10 * (ks - 2)) & 1023u);
+    return 0;
+}
+// Few tiles: the pairs of a cluster share a tile and split its K, as many as leave each 512 values of it and let all
+// clusters run at once (33, 22 and 15 of 2, 3 and 4 pairs on a B200). 128 rows, K = 4096: 15 tiles 18.3 us with two, 13.0
+// with four; 16 tiles 24.6 with one, 18.3 with two, 15.0 with three, 24.2 with four, which do not all fit; 34 tiles 24.8 with
+// one, 35.8 with two.
+int k_splits(long tiles, int np, const Fits& f) {
+    for (int ks = 4; ks > 1; --ks)
+        if (tiles <= f.of[ks] && np >= 8 * ks) return ks;
+    return 1;
 }
 
 template <typename T, int TN, int GROUP>
-int launch_pair_g(const Q4GemmArgs& a, const void* X, long ldx, int rows, long kx, int plane, cudaStream_t st) {
+int launch_pair_g(const Q4GemmArgs& a, const void* X, long ldx, int rows, long kx, int plane, int ks, cudaStream_t st) {
     constexpr int SL = sizeof(T) == 4 ? 3 : 1;
     using C_ = Cfg<SL, TN>;
     PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
@@ -578,7 +616,7 @@ int launch_pair_g(const Q4GemmArgs& a, const void* X, long ldx, int rows, long k
     if (e0) return e0;
     // with offsets the number of tiles is known on the device only: at most one partly filled tile per expert
     const long tiles = tile_count(a, TN);
-    p.ks = TN <= 128 ? k_splits(tiles, p.np, a.num_sms) : 1;
+    p.ks = ks;
     p.span = (p.np / 2 + p.ks - 1) / p.ks * 2;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
@@ -599,10 +637,10 @@ int launch_pair_g(const Q4GemmArgs& a, const void* X, long ldx, int rows, long k
 }
 
 template <typename T, int TN>
-int launch_pair(const Q4GemmArgs& a, const void* X, long ldx, int rows, long kx, int plane, cudaStream_t st) {
-    if (a.group == 32) return launch_pair_g<T, TN, 32>(a, X, ldx, rows, kx, plane, st);
-    if (a.group == 64) return launch_pair_g<T, TN, 64>(a, X, ldx, rows, kx, plane, st);
-    return launch_pair_g<T, TN, 128>(a, X, ldx, rows, kx, plane, st);
+int launch_pair(const Q4GemmArgs& a, const void* X, long ldx, int rows, long kx, int plane, int ks, cudaStream_t st) {
+    if (a.group == 32) return launch_pair_g<T, TN, 32>(a, X, ldx, rows, kx, plane, ks, st);
+    if (a.group == 64) return launch_pair_g<T, TN, 64>(a, X, ldx, rows, kx, plane, ks, st);
+    return launch_pair_g<T, TN, 128>(a, X, ldx, rows, kx, plane, ks, st);
 }
 
 template <typename T>
@@ -629,10 +667,12 @@ int launch_t(const Q4GemmArgs& a, cudaStream_t st) {
     // for 256 (0.49 against 0.375 us at 8192 x 8192).
     const int pairs = a.num_sms / 2, np = (int)((a.K + 127) / 128 * 2);
     const long t128 = tile_count(a, 128), t256 = tile_count(a, 256);
-    const int ks = k_splits(t128, np, a.num_sms);
+    Fits fits;
+    if (const int e = cluster_fits<T>(fits)) return e;
+    const int ks = k_splits(t128, np, fits);
     const double c128 = (double)((t128 * ks + pairs - 1) / pairs) / ks, c256 = 1.3 * (double)((t256 + pairs - 1) / pairs);
-    if (c256 <= c128) return launch_pair<T, 256>(a, X, ldx, rows, kx, plane, st);
-    return launch_pair<T, 128>(a, X, ldx, rows, kx, plane, st);
+    if (c256 <= c128) return launch_pair<T, 256>(a, X, ldx, rows, kx, plane, 1, st);
+    return launch_pair<T, 128>(a, X, ldx, rows, kx, plane, ks, st);
 }
 
 }  // namespace

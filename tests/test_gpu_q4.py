@@ -162,6 +162,14 @@ def test_product_k_splits(cuda, handle, kind, M, N, K, group):
     check_product(cuda, handle, M, N, K, group, kind)
 
 
+@pytest.mark.parametrize("kind", ["fp32", "fp16"])
+@pytest.mark.parametrize("M,N,K,group", [(61, 4096, 1536, 128), (128, 4900, 1700, 64), (49, 5600, 2100, 32), (100, 3800, 2048, 64),
+                                         (128, 5700, 1536, 128), (66, 8400, 1050, 64)])
+def test_product_three_k_splits(cuda, handle, kind, M, N, K, group):
+    """As many tiles as clusters of four, three or two pairs just fit, and one more."""
+    check_product(cuda, handle, M, N, K, group, kind)
+
+
 @pytest.mark.parametrize("kind", ["fp16", "bf16"])
 @pytest.mark.parametrize("M,N,K,group", [(300, 8, 128, 32), (150, 104, 200, 64), (1000, 2008, 256, 128), (777, 1288, 65, 128)])
 def test_product_wide_stores(cuda, handle, kind, M, N, K, group):
