@@ -2,6 +2,7 @@
 #include "q4_common.cuh"
 
 #include <algorithm>
+#include <mutex>
 #include <type_traits>
 
 namespace emu {
@@ -625,16 +626,46 @@ __global__ void __launch_bounds__(32 * kWarps, CTAS) k_q4_rows(RowsParams p) {
     }
 }
 
+__global__ void k_cluster_probe() {}   // never launched: what cluster_fits asks about, with shared memory for 1 to 3 CTAs per SM
+
+// CTAs of a cluster that split K, among those whose clusters all run at once, by the work on the busiest SM: a CTA's units
+// of 128 values of K per warp, 1.8 times as long for two CTAs on an SM and 2.5 for three, and about five units' time for
+// what a CTA does besides. Of equals the larger cluster. Rows x N, K = 4096, groups of 128, against powers of two up to two
+// CTAs per SM: 8 x 9216 11.7 -> 8.6 us (7 CTAs), 16 x 5120 9.8 -> 8.6 (6), 48 x 5120 20.1 -> 16.5 (6), 48 x 9216 30.8 -> 25.8 (2).
+int k_cluster(long clusters, long K, int step, int wk, int most_per_sm, const ClusterFits& fits) {
+    const int slowed[4] = {0, 10, 18, 25};
+    int best = 1;
+    long least = 0;
+    for (int ck = 1; ck <= 8 && (ck == 1 || K >= (long)ck * step); ++ck) {
+        const long units = ((K + ck - 1) / ck + 128L * wk - 1) / (128L * wk);
+        int per_sm = 1;
+        while (per_sm < most_per_sm && clusters > fits.of[per_sm][ck]) ++per_sm;
+        if (ck > 1 && clusters > fits.of[per_sm][ck]) continue;
+        const long cost = 50 + units * slowed[per_sm];
+        if (ck == 1 || cost <= least) {
+            least = cost;
+            best = ck;
+        }
+    }
+    return best;
+}
+
 template <typename T, int NT, int WR, int RBW, int D, int CTAS, int GROUP>
 int launch_rows_g(RowsParams p, int num_sms, cudaStream_t st) {
     constexpr int SL = sizeof(T) == 4 ? 3 : 1;
     constexpr int STEP = kWarps / WR * D * 128;                // values of K that the warps hold in flight
     const long groups = (p.l.nb + WR * RBW - 1) / (WR * RBW);
     const int experts = p.offsets ? std::min(p.E, p.R) : 1;
-    // K split over a cluster while all CTAs are resident at once and each keeps a step of its warps; single rows only below
-    // one CTA per SM (a cluster of two takes about 2 us longer to launch than its CTAs alone)
+    const ClusterFits* fits = cluster_fits();
+    if (!fits) return (int)cudaErrorUnknown;
+    // single rows: only while there is an SM for every CTA (a cluster of two takes about 2 us longer to launch than its
+    // CTAs alone)
     int ck = 1;
-    while (ck < 8 && groups * experts * ck * 2 <= (long)(NT == 1 && WR == 1 ? 1 : CTAS) * num_sms && p.K >= 2L * ck * STEP) ck *= 2;
+    if (NT == 1 && WR == 1) {
+        while (ck < 8 && groups * experts * ck * 2 <= num_sms && p.K >= 2L * ck * STEP) ck *= 2;
+    } else {
+        ck = k_cluster(groups * experts, p.K, STEP, kWarps / WR, CTAS, *fits);
+    }
     p.kspan = (int)(((p.K + ck - 1) / ck + 127) / 128 * 128);
     ck = (int)((p.K + p.kspan - 1) / p.kspan);
     const int cols = SL * std::min(p.R, 8 * NT / SL);
@@ -699,6 +730,38 @@ int launch_rows_t(const RowsParams& p, int group, int num_sms, cudaStream_t st) 
 }
 
 }  // namespace
+
+const ClusterFits* cluster_fits() {
+    static ClusterFits known[64];
+    static std::atomic<unsigned long long> have{0};
+    static std::mutex lock;
+    static thread_local ClusterFits other;           // devices past 64
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (have.load(std::memory_order_acquire) & bit)) return &known[dev];
+    std::lock_guard<std::mutex> hold(lock);
+    ClusterFits& f = dev < 64 ? known[dev] : other;
+    if (dev < 64 && (have.load(std::memory_order_acquire) & bit)) return &f;
+    if (cudaFuncSetAttribute(k_cluster_probe, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) return nullptr;
+    for (int per_sm = 1; per_sm <= 3; ++per_sm)
+        for (int ctas = 1; ctas <= 8; ++ctas) {
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = ctas;
+            attr[0].val.clusterDim.y = 1;
+            attr[0].val.clusterDim.z = 1;
+            cfg.gridDim = dim3(ctas, 1, 1);
+            cfg.blockDim = dim3(256, 1, 1);
+            cfg.dynamicSmemBytes = 200 * 1024 / per_sm;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&f.of[per_sm][ctas], k_cluster_probe, &cfg) != cudaSuccess) return nullptr;
+        }
+    if (dev < 64) have.fetch_or(bit, std::memory_order_release);
+    return &f;
+}
 
 size_t q4_bytes(int E, int N, long K, int group) { return layout(E, N, K, group).bytes; }
 

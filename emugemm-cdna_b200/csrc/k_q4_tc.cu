@@ -538,49 +538,13 @@ __global__ void __launch_bounds__(256) k_q4_stage(const T* __restrict__ A, long 
 long tile_count(const Q4GemmArgs& a, int TN) {
     return ((a.offsets ? std::min(a.E, a.R) : 0) + ((long)a.R + TN - 1) / TN) * ((a.N + 255) / 256);
 }
-// How many clusters of 2, 3 and 4 pairs the device holds at once (a pair keeps two SMs; SMs left over in a GPC hold none).
-struct Fits { int of[5]; };
-template <typename T>
-int cluster_fits(Fits& f) {
-    static std::atomic<unsigned> known[64];          // 10 bits each, per device
-    int dev = 0;
-    const cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return (int)e;
-    unsigned k = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0u;
-    if (!k) {
-        auto kern = k_q4_pair<T, 128, 128>;          // the others take as many threads and (nearly) as much shared memory
-        constexpr int smem = Cfg<sizeof(T) == 4 ? 3 : 1, 128>::SMEM;
-        const cudaError_t a = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (a != cudaSuccess) return (int)a;
-        for (int ks = 2; ks <= 4; ++ks) {
-            cudaLaunchConfig_t cfg = {};
-            cudaLaunchAttribute attr[1];
-            attr[0].id = cudaLaunchAttributeClusterDimension;
-            attr[0].val.clusterDim.x = 2 * ks;
-            attr[0].val.clusterDim.y = 1;
-            attr[0].val.clusterDim.z = 1;
-            cfg.gridDim = dim3(2 * ks, 1, 1);
-            cfg.blockDim = dim3(kThreads, 1, 1);
-            cfg.dynamicSmemBytes = smem;
-            cfg.attrs = attr;
-            cfg.numAttrs = 1;
-            int n = 0;
-            const cudaError_t o = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
-            if (o != cudaSuccess) return (int)o;
-            k |= (unsigned)std::min(n, 1023) << (10 * (ks - 2));
-        }
-        if (dev < 64) known[dev].store(k | 1u << 30, std::memory_order_relaxed);
-    }
-    for (int ks = 2; ks <= 4; ++ks) f.of[ks] = (int)(k >> (10 * (ks - 2)) & 1023u);
-    return 0;
-}
 // Few tiles: the pairs of a cluster share a tile and split its K, as many as leave each 512 values of it and let all
 // clusters run at once (33, 22 and 15 of 2, 3 and 4 pairs on a B200). 128 rows, K = 4096: 15 tiles 18.3 us with two, 13.0
 // with four; 16 tiles 24.6 with one, 18.3 with two, 15.0 with three, 24.2 with four, which do not all fit; 34 tiles 24.8 with
 // one, 35.8 with two.
-int k_splits(long tiles, int np, const Fits& f) {
+int k_splits(long tiles, int np, const ClusterFits& f) {
     for (int ks = 4; ks > 1; --ks)
-        if (tiles <= f.of[ks] && np >= 8 * ks) return ks;
+        if (tiles <= f.of[1][2 * ks] && np >= 8 * ks) return ks;
     return 1;
 }
 
@@ -667,9 +631,9 @@ int launch_t(const Q4GemmArgs& a, cudaStream_t st) {
     // for 256 (0.49 against 0.375 us at 8192 x 8192).
     const int pairs = a.num_sms / 2, np = (int)((a.K + 127) / 128 * 2);
     const long t128 = tile_count(a, 128), t256 = tile_count(a, 256);
-    Fits fits;
-    if (const int e = cluster_fits<T>(fits)) return e;
-    const int ks = k_splits(t128, np, fits);
+    const ClusterFits* fits = cluster_fits();
+    if (!fits) return (int)cudaErrorUnknown;
+    const int ks = k_splits(t128, np, *fits);
     const double c128 = (double)((t128 * ks + pairs - 1) / pairs) / ks, c256 = 1.3 * (double)((t256 + pairs - 1) / pairs);
     if (c256 <= c128) return launch_pair<T, 256>(a, X, ldx, rows, kx, plane, 1, st);
     return launch_pair<T, 128>(a, X, ldx, rows, kx, plane, ks, st);

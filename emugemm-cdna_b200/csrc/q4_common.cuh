@@ -37,6 +37,11 @@ struct OncePerDevice {
     }
 };
 
+// Clusters that the current device holds at once, by CTAs resident on an SM (1 .. 3) and CTAs per cluster (1 .. 8): fewer
+// than the SMs would make, since a cluster stays within one GPC. Null: a CUDA error.
+struct ClusterFits { int of[4][9]; };
+const ClusterFits* cluster_fits();   // k_q4.cu
+
 namespace q4 {
 
 struct Layout {
