@@ -45,10 +45,16 @@ emugemm_status_t q4_product(emugemm_handle_t handle, int R, int E, int N, long K
     a.err = h->err_dev;
     const int with = experts ? (E < R ? E : R) : 1;   // experts that can have rows
     const long cols = (long)(R / with) * (dtype == EMU_DTYPE_F32 ? 3 : 1);
-    // Few columns: one pass over the codes per 48 of them (k_q4.cu), else tiles of CTA pairs (k_q4_tc.cu). 8192 x 8192,
-    // groups of 128: 48 columns 37 against 34 us, 64 (two passes) 64 against 34; 4096 x 4096: 14 against 23 and 23 against
-    // 23. Groups of 32 cost the tiles an accumulator each, the passes nothing: 64 columns 27 against 41 us.
-    if (cols <= (group == 32 ? 96 : 48)) {
+    // Few columns: one pass over the codes per 48 of them (k_q4.cu), else tiles of CTA pairs (k_q4_tc.cu), in us:
+    //   48 columns, groups of 128:  4096 x 4096 13.7 against 15.0, 8192 x 4096 20.3 / 19.0, 8192 x 8192 35.4 / 29.4
+    //   32 columns, groups of 128:  8192 x 8192 26.1 / 28.8;  48 columns, groups of 64:  11008 x 4096 29.8 / 37.8
+    //   16 rows FP32 (48 columns):  4096 x 4096 13.1 / 19.4;  64 columns, groups of 128:  4096 x 4096 23 / 15
+    //   groups of 32, an accumulator each on the tiles:  64 columns, 4096 x 4096 25.7 / 27.6, 8192 x 8192 74.5 / 82.6,
+    //   11008 x 4096 56.5 / 69.7;  96 columns 29.2 / 27.8, 83.3 / 83.2, 64.6 / 70.9;  2048 x 2048: 17.3 / 14.4, 20.0 / 14.4
+    const long weights = (long)with * N * K;
+    const bool large = group == 128 && dtype != EMU_DTYPE_F32 && !experts && weights >= (1L << 25);
+    const long most = group == 32 && weights >= (1L << 24) ? 96 : large ? 32 : 48;
+    if (cols <= most) {
         ProfScope ps(h, kProfQ4);
         return from_cuda(launch_q4_rows(a, h->stream));
     }
