@@ -4,6 +4,10 @@ Bars: packing and unpacking bit for bit; products within q4ref.product_bound, wh
 the FP32 accumulation; the same call twice bit for bit."""
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -408,6 +412,37 @@ def test_capture_and_replay_with_new_inputs(cuda, M, kind):
             assert torch.equal(c, want)
         h.sync()
         del graph
+
+
+@pytest.mark.parametrize("M", [1, 20, 100])
+def test_first_call_of_a_process_inside_a_capture(cuda, M):
+    """Nothing that a call does once per process or device is closed to a capture."""
+    code = f"""
+import torch, emugemm, q4ref
+M, N, K, group = {M}, 520, 2048, 64
+s = torch.cuda.Stream()
+h = emugemm.Handle(s)
+packed, w = q4ref.weights(3, 1, N, K, group)
+x = torch.ones(M, K, dtype=torch.bfloat16, device="cuda")
+y = torch.full((M, N), -7.5, dtype=torch.bfloat16, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    h.q4_gemm(M, N, K, x, K, packed, group, y, N)
+assert (y == -7.5).all()
+g.replay()
+torch.cuda.synchronize()
+h.sync()
+xd = x.double().cpu().numpy()
+ref = xd @ w[0].T
+assert (abs(y.double().cpu().numpy() - ref) <= q4ref.product_bound(xd, w[0], ref, group, "bf16")).all()
+print("right")
+"""
+    here = os.path.dirname(os.path.abspath(__file__))
+    path = os.pathsep.join([here, os.path.dirname(os.path.abspath(emugemm.__file__)), os.environ.get("PYTHONPATH", "")])
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": path}, capture_output=True, text=True,
+                       timeout=120)
+    assert r.returncode == 0 and "right" in r.stdout, r.stderr[-2000:]
 
 
 def test_capture_needs_the_workspace_first(cuda):
