@@ -34,14 +34,19 @@ emugemm_status_t from_cuda(int e) {
     return EMUGEMM_STATUS_INTERNAL_ERROR;
 }
 
+// Bytes the handle holds besides those of `slot` (-1: of no slot): the other slots and what captured graphs keep.
+static size_t ws_others(const Handle* h, int slot) {
+    size_t total = 0;
+    for (int i = 0; i < kWsCount; ++i) total += (i == slot) ? 0 : h->ws_size[i];
+    for (const Handle::Retired* r = h->retired; r; r = r->next) total += r->bytes;
+    return total;
+}
+
 // Grow-only workspace slot (src/emugemm.cpp:79-87, but per handle and with an optional cap).
 void* ws_get(Handle* h, int slot, size_t bytes) {
     if (bytes == 0) bytes = 256;
     if (h->ws_size[slot] >= bytes) return h->ws[slot];
-    size_t total = 0;
-    for (int i = 0; i < kWsCount; ++i) total += (i == slot) ? 0 : h->ws_size[i];
-    for (const Handle::Retired* r = h->retired; r; r = r->next) total += r->bytes;
-    if (h->ws_limit && total + bytes > h->ws_limit) return nullptr;
+    if (h->ws_limit && ws_others(h, slot) + bytes > h->ws_limit) return nullptr;
     if (h->ws[slot]) {
         cudaStreamSynchronize((cudaStream_t)h->stream);
         cudaFree(h->ws[slot]);
@@ -68,16 +73,24 @@ void* ws_get_kept(Handle* h, int slot, size_t bytes) {
         h->ws_kept[slot] = true;
         return h->ws[slot];
     }
-    if (h->ws_size[slot] < bytes && h->ws_kept[slot]) {
-        Handle::Retired* r = (Handle::Retired*)std::malloc(sizeof(Handle::Retired));
-        if (!r) return nullptr;
-        *r = Handle::Retired{h->ws[slot], h->ws_size[slot], h->retired};
-        h->retired = r;
-        h->ws[slot] = nullptr;
-        h->ws_size[slot] = 0;
-        h->ws_kept[slot] = false;
+    if (h->ws_size[slot] >= bytes || !h->ws_kept[slot]) return ws_get(h, slot, bytes);
+    // new memory beside the kept one, which the slot gives up only once the new is there: a refused call leaves the handle
+    // as it was
+    if (h->ws_limit && ws_others(h, -1) + bytes > h->ws_limit) return nullptr;
+    Handle::Retired* r = (Handle::Retired*)std::malloc(sizeof(Handle::Retired));
+    if (!r) return nullptr;
+    void* p = nullptr;
+    if (cudaMalloc(&p, bytes) != cudaSuccess) {
+        cudaGetLastError();
+        std::free(r);
+        return nullptr;
     }
-    return ws_get(h, slot, bytes);
+    *r = Handle::Retired{h->ws[slot], h->ws_size[slot], h->retired};
+    h->retired = r;
+    h->ws[slot] = p;
+    h->ws_size[slot] = bytes;
+    h->ws_kept[slot] = false;
+    return p;
 }
 
 DeviceGuard::DeviceGuard(int dev) {
