@@ -584,6 +584,14 @@ emugemm_status_t emugemm_set_stream(emugemm_handle_t handle, void* stream) {
     return EMUGEMM_STATUS_SUCCESS;
 }
 
+emugemm_status_t emugemm_get_device(emugemm_handle_t handle, int* device) {
+    Handle* h = reinterpret_cast<Handle*>(handle);
+    if (!h) return EMUGEMM_STATUS_INVALID_HANDLE;
+    if (!device) return EMUGEMM_STATUS_INVALID_POINTER;
+    *device = h->device;
+    return EMUGEMM_STATUS_SUCCESS;
+}
+
 emugemm_status_t emugemm_set_workspace_limit(emugemm_handle_t handle, size_t bytes) {
     Handle* h = reinterpret_cast<Handle*>(handle);
     if (!h) return EMUGEMM_STATUS_INVALID_HANDLE;

@@ -11,7 +11,6 @@ import ctypes
 import os
 import pathlib
 import re
-import sys
 
 HERE = pathlib.Path(__file__).resolve().parent
 LIB_PATH = HERE / "libemugemm.so"
@@ -82,6 +81,7 @@ _SIGS = {
     "emugemm_create_handle": (c_int, [P(c_void_p)]),
     "emugemm_destroy_handle": (c_int, [c_void_p]),
     "emugemm_set_stream": (c_int, [c_void_p, c_void_p]),
+    "emugemm_get_device": (c_int, [c_void_p, P(c_int)]),
     "emugemm_set_workspace_limit": (c_int, [c_void_p, c_size_t]),
     "emugemm_sync": (c_int, [c_void_p]),
     "emugemm_init": (c_int, [ctypes.c_char_p]),
@@ -237,8 +237,9 @@ class Handle:
         h = c_void_p()
         check("emugemm_create_handle", lib().emugemm_create_handle(ctypes.byref(h)))
         self.h = h
-        torch = sys.modules.get("torch")
-        self.device = torch.cuda.current_device() if torch is not None else None   # of the tensors it may be given
+        device = c_int()
+        check("emugemm_get_device", lib().emugemm_get_device(h, ctypes.byref(device)))
+        self.device = device.value   # of the tensors it may be given
         if stream is not None:
             self.set_stream(stream)
         # kernel choices as created (from the environment), restored by reset_kernels()
@@ -408,7 +409,7 @@ class Handle:
         dtype (ValueError): a kernel given a host address or another type's bytes would fault or compute nonsense."""
         if x is None or isinstance(x, int):
             return x or 0
-        if self.device is not None and x.get_device() != self.device:
+        if x.get_device() != self.device:
             raise ValueError(f"expected a tensor on cuda:{self.device}, got one on {x.device}")
         if name is not None:
             d = x.dtype

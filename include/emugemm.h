@@ -98,6 +98,8 @@ emugemm_status_t emugemm_destroy_handle(emugemm_handle_t handle);
 /* All work of the handle is enqueued on `stream` (a cudaStream_t; NULL = legacy default stream).
    Replaces rocblas_set_stream. */
 emugemm_status_t emugemm_set_stream(emugemm_handle_t handle, void* stream);
+/* The device the handle was created on (a CUDA device ordinal): the one its calls run on and its buffers must lie on. */
+emugemm_status_t emugemm_get_device(emugemm_handle_t handle, int* device);
 /* Caps the handle's grow-only workspace; 0 = no cap. A call needing more returns MEMORY_ERROR. */
 emugemm_status_t emugemm_set_workspace_limit(emugemm_handle_t handle, size_t bytes);
 
