@@ -99,7 +99,8 @@ __global__ void __launch_bounds__(256, 4) k_q4_pack(const T* __restrict__ W, lon
             const T* row = W + ((size_t)e * N + n) * ldw;
 #pragma unroll
             for (int gi = 0; gi < 4 / PER; ++gi) {
-                float v[PER][8];
+                __align__(16) float v[PER][8];
+                static_assert(__alignof__(v) >= 16, "written 16 bytes at a time");
 #pragma unroll
                 for (int i = 0; i < PER; ++i) {
                     const long k = k128 * 128 + GROUP * gi + 32 * i + 8 * t;

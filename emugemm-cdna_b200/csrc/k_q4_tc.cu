@@ -514,7 +514,8 @@ __global__ void __launch_bounds__(256) k_q4_stage(const T* __restrict__ A, long 
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
         const long m = i / chunks, k = (i - m * chunks) * 8;
         const T* a = A + (size_t)m * lda + k;
-        T x[8];
+        __align__(16) T x[8];
+        static_assert(__alignof__(x) >= 16, "written and read 16 bytes at a time");
         if (sizeof(T) == 4 && vec && k + 8 <= K) {
             reinterpret_cast<float4*>(x)[0] = reinterpret_cast<const float4*>(a)[0];
             reinterpret_cast<float4*>(x)[1] = reinterpret_cast<const float4*>(a)[1];
