@@ -252,6 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
         }
         if (lane == 0) first[p.E] = run;
     }
+    __syncwarp();                                  // the barriers below are .aligned: whole warps
     tc_fence_before();
     cluster_sync_all();
     tc_fence_after();
@@ -502,6 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
                         c[(size_t)(j + i) * p.ldc] = from_float<T>((v[0][i] + v[1][i] + v[2][i] + v[3][i]) * code_unit<BF16>());
             }
         }
+        __syncwarp();                              // lanes behind column N - 1 left the loop early
         cluster_sync_all();                        // no CTA leaves while its parts are read
     }
 }
