@@ -284,11 +284,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
                         tma_load_2d_pair(st + sl * C_::PANEL_B, &tm_x, fb, (p0 + k) * 64, sl * p.plane + row);
                 }
             }
+            // The leader's last commits arrive here, also those of stages that nobody waits for again: no CTA leaves before
+            // they have. Where a role gave up, the loads in flight are waited for instead.
+            const long last = it > ST ? it - ST : 0;
+            for (long j = last; j < it && ok; ++j)
+                ok = wait(&ctl->empty[j % ST], (uint32_t)((j / ST) & 1), abort, p.err, kErrTimeoutProducer);
             if (!ok) {
                 abort_pair(ctl, peer);
                 if (leader)
-                    for (long j = it > ST ? it - ST : 0; j < it; ++j)
-                        drain_wait(&ctl->full[j % ST], (uint32_t)((j / ST) & 1));
+                    for (long j = last; j < it; ++j) drain_wait(&ctl->full[j % ST], (uint32_t)((j / ST) & 1));
             }
         } else if (warp == 1 && leader) {
             // ---------------- leader: pair MMA issuer ----------------
