@@ -1,10 +1,17 @@
-"""4-bit products on the GPU, what the other files leave of their range: workspaces that captured graphs keep."""
+"""4-bit products on the GPU, what the other files leave of their range: workspaces that captured graphs keep, and row tiles
+of both heights with more tiles than CTA pairs.
+
+Bars: q4ref.product_bound."""
 from __future__ import annotations
 
+import functools
+
+import numpy as np
 import pytest
 
 import emugemm
 import q4ref
+from q4ref import TYPES
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +57,77 @@ def test_refused_growth_keeps_what_a_graph_uses(cuda):
         h.sync()
         assert torch.equal(c, want)
         del graphs, g
+
+
+# ------------------------------------------------------------------------------------------- row tiles of both heights
+def tile_rows(torch, R, N, experts=0):
+    """(rows of A per tile, tiles) by the launch's rule for products of many rows whose K is not split: rounds of the CTA
+    pairs, 1.3 times as long for 256 rows. With experts one tile more for each, which the host cannot rule out."""
+    pairs = torch.cuda.get_device_properties(0).multi_processor_count // 2
+    tiles = {h: (experts + -(-R // h)) * -(-N // 256) for h in (128, 256)}
+    rounds = {h: -(-tiles[h] // pairs) for h in tiles}
+    return (256, tiles[256]) if 1.3 * rounds[256] <= rounds[128] else (128, tiles[128])
+
+
+@functools.lru_cache(maxsize=None)
+def layer(E, N, K, group):
+    return q4ref.weights(E * N + K, E, N, K, group)
+
+
+def close(got, x, w, group, kind):
+    ref = x @ w.T
+    bad = ~(np.abs(got - ref) <= q4ref.product_bound(x, w, ref, group, kind))     # NaN is bad, too
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4], np.nanmax(np.abs(got - ref)))
+
+
+# One tile per pair and several; K of one panel, of odd counts, and of more panels than the shared memory has stages
+MANY = [(2100, 1200, 200, 256, False), (2400, 1999, 1100, 256, True), (2560, 2048, 64, 256, True), (100, 19300, 330, 128, True),
+        (5000, 4000, 70, 256, True)]
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K,height,several", MANY)
+def test_product_of_many_tiles(cuda, handle, kind, group, M, N, K, height, several):
+    torch = cuda
+    rows, tiles = tile_rows(torch, M, N)
+    pairs = torch.cuda.get_device_properties(0).multi_processor_count // 2
+    assert rows == height and (tiles > pairs) == several        # the case is what it stands for
+    packed, w = layer(1, N, K, group)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(TYPES[kind])
+    c = torch.full((M + 1, N), -7.5, dtype=TYPES[kind], device="cuda")
+    handle.q4_gemm(M, N, K, x.cuda(), K, packed, group, c, N)
+    handle.sync()
+    got = c.double().cpu().numpy()
+    assert (got[M] == -7.5).all()
+    close(got[:M], x.double().numpy(), w[0], group, kind)
+    c2 = torch.empty_like(c)
+    handle.q4_gemm(M, N, K, x.cuda(), K, packed, group, c2, N)
+    handle.sync()
+    assert torch.equal(c[:M], c2[:M])
+
+
+EXPERTS = [([700, 0, 1300, 3, 256, 257, 0], 1500, 333, 5, 256), ([300, 1, 90, 0, 250, 130], 2600, 200, 0, 128),
+           ([0, 2560, 0], 2048, 130, 40, 256)]
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("counts,N,K,tail,height", EXPERTS)
+def test_experts_of_many_tiles(cuda, handle, kind, group, counts, N, K, tail, height):
+    torch = cuda
+    E, off = len(counts), np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    used, R = int(off[-1]), int(off[-1]) + tail
+    assert tile_rows(torch, R, N, E)[0] == height
+    pairs = torch.cuda.get_device_properties(0).multi_processor_count // 2
+    assert sum(-(-n // height) for n in counts) * -(-N // 256) > pairs      # a pair takes more than one tile
+    packed, w = layer(E, N, K, group)
+    x = torch.randn(R, K, generator=torch.Generator().manual_seed(R)).to(TYPES[kind])
+    c = torch.full((R + 1, N), -7.5, dtype=TYPES[kind], device="cuda")
+    handle.q4_gemm_experts(R, E, N, K, x.cuda(), K, torch.from_numpy(off).cuda(), packed, group, c, N)
+    handle.sync()
+    got, xd = c.double().cpu().numpy(), x.double().numpy()
+    assert (got[used:] == -7.5).all()
+    for e in range(E):
+        if counts[e]:
+            close(got[off[e]:off[e + 1]], xd[off[e]:off[e + 1]], w[e], group, kind)
