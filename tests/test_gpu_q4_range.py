@@ -131,3 +131,64 @@ def test_experts_of_many_tiles(cuda, handle, kind, group, counts, N, K, tail, he
     for e in range(E):
         if counts[e]:
             close(got[off[e]:off[e + 1]], xd[off[e]:off[e + 1]], w[e], group, kind)
+
+
+# ------------------------------------------------------------------------------------------------ 24 bits of FP32 rows
+def one_value_rows(rows, K, seed):
+    """Rows of zeros with one value each, whose 24 significant bits end in a byte of 64 or more: without the lowest slice
+    it is off by at least 2^-18 of itself. The places k run over all of K."""
+    g = np.random.default_rng(seed)
+    k = (g.permutation(rows) * K // rows + g.integers(0, max(1, K // rows), rows)).clip(max=K - 1)
+    m = (g.integers(2 ** 15, 2 ** 16, rows) * 256 + g.integers(64, 256, rows)).astype(np.float64)
+    x = np.zeros((rows, K), np.float32)
+    x[np.arange(rows), k] = m * 2.0 ** (g.integers(-3, 4, rows) - 23) * g.choice([-1, 1], rows)
+    return x
+
+
+def check_low_bits(got, x, w):
+    """C is scale * q * x of one place, the rest adds zeros: the sum of the three slices' products loses at most one step
+    of 2^-23 in the tensor cores, which truncate, and each of the multiplication by the scale and the two additions of
+    slices kept apart rounds by 2^-24 at most (a kernel does one or the other)."""
+    ref = x.astype(np.float64) @ w.T
+    bad = ~(np.abs(got - ref) <= 3 * 2.0 ** -24 * np.abs(ref))
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4], np.nanmax(np.abs(got - ref) / np.abs(ref)))
+
+
+# The column tiles of few rows, K splits over pairs, and row tiles of 128 and 256; K with a last group that is not whole
+LOW = [(1, 40, 2052), (1, 700, 4096), (2, 300, 1300), (4, 130, 1028), (8, 260, 1500), (10, 100, 2052), (16, 300, 1100),
+       (60, 130, 1036), (100, 300, 2200), (128, 520, 4100), (400, 640, 1088), (2100, 1200, 200), (2400, 1999, 260)]
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", LOW)
+@pytest.mark.parametrize("gap", [0, 1])
+def test_product_keeps_the_low_bits(cuda, handle, group, M, N, K, gap):
+    """gap: a leading dimension that breaks the rows' alignment."""
+    torch = cuda
+    packed, w = layer(1, N, K, group)
+    for seed in range(max(1, 24 // M)):
+        x = one_value_rows(M, K, 100 * seed + M) if M > 1 else one_value_rows(24, K, M)[seed:seed + 1]
+        a = torch.full((M, K + gap), float("nan"), device="cuda")
+        a[:, :K] = torch.from_numpy(x).cuda()
+        c = torch.empty(M, N, device="cuda")
+        handle.q4_gemm(M, N, K, a, K + gap, packed, group, c, N)
+        handle.sync()
+        check_low_bits(c.double().cpu().numpy(), x, w[0])
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("counts,N,K", [([3, 0, 1, 9, 0, 2], 100, 332), ([40, 1, 0, 130], 160, 1052), ([60, 70, 0, 90], 200, 2100),
+                                        ([700, 0, 1300, 3, 256, 257, 0], 1500, 332)])
+def test_experts_keep_the_low_bits(cuda, handle, group, counts, N, K):
+    torch = cuda
+    E, off = len(counts), np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    R = int(off[-1])
+    packed, w = layer(E, N, K, group)
+    x = one_value_rows(R, K, R)
+    c = torch.empty(R, N, device="cuda")
+    handle.q4_gemm_experts(R, E, N, K, torch.from_numpy(x).cuda(), K, torch.from_numpy(off).cuda(), packed, group, c, N)
+    handle.sync()
+    got = c.double().cpu().numpy()
+    for e in range(E):
+        if counts[e]:
+            check_low_bits(got[off[e]:off[e + 1]], x[off[e]:off[e + 1]], w[e])
