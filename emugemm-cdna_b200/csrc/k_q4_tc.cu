@@ -512,11 +512,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_q4_pair(const __grid_constant__
     }
 }
 
-// Rows of A as TMA can read them: 16-bit rows of Kp values (zeros behind K), FP32 rows as three planes of bf16 slices.
+// Rows of A as TMA can read them: 16-bit rows of Kp values (zeros behind K), FP32 rows as three planes of bf16 slices. With
+// offsets only up to the last row that an expert claims (the largest offset: the last one, unless they run backwards).
 template <typename T>
 __global__ void __launch_bounds__(256) k_q4_stage(const T* __restrict__ A, long lda, int R, long K, long Kp,
-                                                  uint16_t* __restrict__ X, int vec) {
-    const long chunks = Kp / 8, n = (long)R * chunks;
+                                                  uint16_t* __restrict__ X, int vec, const int* __restrict__ offsets, int E) {
+    __shared__ int claimed[8];
+    int rows = R;
+    if (offsets) {
+        rows = 0;
+        for (int e = threadIdx.x; e < E; e += 256) rows = max(rows, min(R, __ldg(offsets + e + 1)));
+        __syncwarp();
+        rows = __reduce_max_sync(0xffffffffu, rows);
+        if ((threadIdx.x & 31) == 0) claimed[threadIdx.x >> 5] = rows;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 8; ++w) rows = max(rows, claimed[w]);
+    }
+    const long chunks = Kp / 8, n = rows * chunks;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
         const long m = i / chunks, k = (i - m * chunks) * 8;
         const T* a = A + (size_t)m * lda + k;
@@ -628,7 +641,7 @@ int launch_t(const Q4GemmArgs& a, cudaStream_t st) {
         const int grid = (int)std::min((n + 255) / 256, 16L * a.num_sms);
         const int vec = (reinterpret_cast<uintptr_t>(a.A) & 15) == 0 && (a.lda * sizeof(T)) % 16 == 0;
         k_q4_stage<T><<<grid, 256, 0, st>>>(static_cast<const T*>(a.A), a.lda, a.R, a.K, kx,
-                                            static_cast<uint16_t*>(a.stage), vec);
+                                            static_cast<uint16_t*>(a.stage), vec, a.offsets, a.E);
         count_launch();
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return (int)e;

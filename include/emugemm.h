@@ -327,7 +327,7 @@ emugemm_status_t emugemm_q4_gemm(emugemm_handle_t handle, int M, int N, long K, 
                                  const void* packed, int group, void* C, long ldc);
 /* The same with weights of E experts: rows offsets[e] .. offsets[e+1] - 1 of A and C (device array of E + 1, not
    decreasing, as made by emugemm_expert_sort) use expert e's weights; the other rows of C, up to R, are left as they
-   were. The work follows the rows that are there, not R. */
+   were. The work follows the rows that are there, not R (what it uses of the workspace follows R). */
 emugemm_status_t emugemm_q4_gemm_experts(emugemm_handle_t handle, int R, int E, int N, long K, const void* A, long lda,
                                          int dtype, const int* offsets, const void* packed, int group, void* C,
                                          long ldc);

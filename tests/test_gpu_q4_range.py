@@ -192,3 +192,45 @@ def test_experts_keep_the_low_bits(cuda, handle, group, counts, N, K):
     for e in range(E):
         if counts[e]:
             check_low_bits(got[off[e]:off[e + 1]], x[off[e]:off[e + 1]], w[e])
+
+
+# ------------------------------------------------------------------------------------------------------ rows not there
+def test_work_follows_the_rows_that_are_there(cuda):
+    """FP32 rows are staged before the product: 64 rows that are there among 262144 are done in a small part of the time of
+    all of them (staging all R takes more than half of it, so a quarter tells the two apart)."""
+    torch = cuda
+    E, R, N, K, group = 4, 1 << 18, 16, 1024, 64
+    packed, w = layer(E, N, K, group)
+    a = torch.randn(R, K, device="cuda")
+    c = torch.full((R, N), -7.5, device="cuda")
+    few, every = ([n * i for i in range(E + 1)] for n in (16, R // E))
+    off = {n: torch.tensor(o, dtype=torch.int32, device="cuda") for n, o in (("few", few), ("all", every))}
+    ms = {}
+    with emugemm.Handle() as h:
+        for name in ("few", "all"):
+            for _ in range(4):
+                h.profile_begin()
+                h.q4_gemm_experts(R, E, N, K, a, K, off[name], packed, group, c, N)
+                ms[name] = min(ms.get(name, 1e9), h.profile_end()["q4"][0])
+            if name == "few":
+                assert (c[64:] == -7.5).all()
+                got, x = c[:64].double().cpu().numpy(), a[:64].double().cpu().numpy()
+                for e in range(E):
+                    close(got[16 * e:16 * e + 16], x[16 * e:16 * e + 16], w[e], group, "fp32")
+    assert ms["few"] < ms["all"] / 4, ms
+
+
+def test_backward_offsets_stage_what_is_claimed(cuda, handle):
+    """Offsets that run backwards: the rows of the experts that do have rows are right, whatever the last offset says."""
+    torch = cuda
+    E, R, N, K, group = 4, 300, 40, 132, 32
+    packed, w = layer(E, N, K, group)
+    a = torch.randn(R, K, generator=torch.Generator().manual_seed(1)).cuda()
+    c = torch.full((R, N), -7.5, device="cuda")
+    off = torch.tensor([0, 120, 260, 250, 3], dtype=torch.int32, device="cuda")      # experts 0 and 1; 2 and 3 have none
+    handle.q4_gemm_experts(R, E, N, K, a, K, off, packed, group, c, N)
+    handle.sync()
+    got, x = c.double().cpu().numpy(), a.double().cpu().numpy()
+    close(got[:120], x[:120], w[0], group, "fp32")
+    close(got[120:260], x[120:260], w[1], group, "fp32")
+    assert (got[260:] == -7.5).all()
