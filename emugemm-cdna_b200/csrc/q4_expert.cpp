@@ -53,7 +53,13 @@ emugemm_status_t q4_product(emugemm_handle_t handle, int R, int E, int N, long K
     //   11008 x 4096 56.5 / 69.7;  96 columns 29.2 / 27.8, 83.3 / 83.2, 64.6 / 70.9;  2048 x 2048: 17.3 / 14.4, 20.0 / 14.4
     const long weights = (long)with * N * K;
     const bool large = group == 128 && dtype != EMU_DTYPE_F32 && !experts && weights >= (1L << 25);
-    const long most = group == 32 && weights >= (1L << 24) ? 96 : large ? 32 : 48;
+    // More than 8 experts: rows are seldom dealt evenly among them, and the passes of 48 columns of the fullest expert follow
+    // one another, so the 96 of groups of 32 do not hold for them (mean rows; even, mildly and strongly uneven):
+    //   16 x 2048 x 4096: 52 rows 136, 186, 376 against 139, 139, 142, 96 rows 159, 284, 667 against 184, 184, 183;  16 x 1024 x
+    //   1024: 64 rows 31, 45, 103 against 23;  32 x 4096 x 2048: 52 rows 251, 223, 268 against 276, 276, 310, 96 rows 302, 379,
+    //   497 against 337, 336, 382;  FP32 16 x 2048 x 4096: 24 rows 149, 204, 495 against 200.  4 x 2048 x 2048: 64 rows 29, 29,
+    //   30 against 36, 96 rows 33, 41, 42 against 37;  8 x 1024 x 4096: 90 rows 48, 64, 71 against 64
+    const long most = group == 32 && weights >= (1L << 24) && with <= 8 ? 96 : large ? 32 : 48;
     if (cols <= most) {
         ProfScope ps(h, kProfQ4);
         return from_cuda(launch_q4_rows(a, h->stream));

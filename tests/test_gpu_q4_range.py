@@ -234,3 +234,28 @@ def test_backward_offsets_stage_what_is_claimed(cuda, handle):
     close(got[:120], x[:120], w[0], group, "fp32")
     close(got[120:260], x[120:260], w[1], group, "fp32")
     assert (got[260:] == -7.5).all()
+
+
+# ------------------------------------------------------------------------------------------------------ rows or tiles
+@pytest.mark.parametrize("E,launches", [(4, 1), (16, 2)])
+def test_many_experts_go_to_tiles(cuda, handle, E, launches):
+    """Groups of 32 with a mean of 60 rows: of more than 8 experts, which are seldom even, on row tiles, where unaligned rows
+    are staged first (two launches); of few experts in passes of 48 columns (one)."""
+    torch = cuda
+    N, K, group = (1 << 24) // (1024 * E) + 8, 1025, 32
+    R = 60 * E
+    w = torch.randn(E * N, K, generator=torch.Generator().manual_seed(E)).bfloat16().cuda()
+    packed = torch.empty(emugemm.q4_bytes(E, N, K, group), dtype=torch.uint8, device="cuda")
+    handle.q4_pack(E, N, K, w, K, group, packed)
+    off = torch.arange(0, R + 1, 60, dtype=torch.int32, device="cuda")
+    x = torch.randn(R, K, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    c = torch.empty(R, N, dtype=torch.bfloat16, device="cuda")
+    before = emugemm.lib().emugemm_kernel_launch_count()
+    handle.q4_gemm_experts(R, E, N, K, x, K, off, packed, group, c, N)
+    assert emugemm.lib().emugemm_kernel_launch_count() - before == launches
+    out = torch.empty(E * N, K, device="cuda")
+    handle.q4_unpack(E, N, K, group, packed, out, K)
+    handle.sync()
+    v, xd = out.view(E, N, K).double().cpu().numpy(), x.double().cpu().numpy()
+    for e in (0, E - 1):
+        close(c[60 * e:60 * e + 60].double().cpu().numpy(), xd[60 * e:60 * e + 60], v[e], group, "bf16")
