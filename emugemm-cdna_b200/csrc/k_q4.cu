@@ -725,7 +725,8 @@ int launch_rows_t(const RowsParams& p, int group, int num_sms, cudaStream_t st) 
         // scales of four groups per unit and two row blocks do not fit the registers beside three column tiles
         // (24 x 5001 x 7013, groups of 32: 23.0 against 20.8 us; 24 x 8192 x 8192, groups of 128: 19.7 against 26.0)
         if (group == 32) return launch_rows_g<T, 3, 8, 1, 1, 3, 32>(p, num_sms, st);
-        return launch_rows_n<T, 3, 8, 2, 1, 2>(p, group, num_sms, st);
+        if (group == 64) return launch_rows_g<T, 3, 8, 2, 1, 2, 64>(p, num_sms, st);
+        return launch_rows_g<T, 3, 8, 2, 1, 2, 128>(p, num_sms, st);
     }
     if (cols <= 32) return launch_rows_n<T, 4, 8, 1, 2, 2>(p, group, num_sms, st);
     return launch_rows_n<T, 6, 8, 1, 2, 2>(p, group, num_sms, st);
