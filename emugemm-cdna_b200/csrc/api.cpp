@@ -29,6 +29,7 @@ void count_launch(unsigned n) { g_launches.fetch_add(n, std::memory_order_relaxe
 
 emugemm_status_t from_cuda(int e) {
     if (e == 0) return EMUGEMM_STATUS_SUCCESS;
+    cudaGetLastError();   // reported here once: the next call must not find it again behind its own launches
     if (e == (int)cudaErrorMemoryAllocation) return EMUGEMM_STATUS_MEMORY_ERROR;
     if (e == (int)cudaErrorInvalidValue) return EMUGEMM_STATUS_INVALID_VALUE;
     return EMUGEMM_STATUS_INTERNAL_ERROR;

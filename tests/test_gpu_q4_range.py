@@ -5,6 +5,9 @@ Bars: q4ref.product_bound."""
 from __future__ import annotations
 
 import functools
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -259,3 +262,53 @@ def test_many_experts_go_to_tiles(cuda, handle, E, launches):
     v, xd = out.view(E, N, K).double().cpu().numpy(), x.double().cpu().numpy()
     for e in (0, E - 1):
         close(c[60 * e:60 * e + 60].double().cpu().numpy(), xd[60 * e:60 * e + 60], v[e], group, "bf16")
+
+
+# -------------------------------------------------------------------------------------------------- after a failed call
+def test_a_failed_launch_is_reported_once(cuda):
+    """A call into a capture that has become invalid fails; the calls after the capture has ended are not blamed for it.
+    (A process of its own: torch does not get over a broken capture.)"""
+    code = """
+import os, torch, emugemm, q4ref
+M, N, K, group = 4, 520, 2048, 64
+s = torch.cuda.Stream()
+h = emugemm.Handle(s)
+packed, w = q4ref.weights(3, 1, N, K, group)
+x = torch.ones(M, K, dtype=torch.bfloat16, device="cuda")
+y = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+def one():
+    h.q4_gemm(M, N, K, x, K, packed, group, y, N)
+one()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+failed = 0
+with torch.cuda.stream(s):
+    g.capture_begin()
+    try:
+        torch.cuda.synchronize()          # not allowed in a capture: it makes the capture invalid
+    except RuntimeError:
+        failed += 1
+    try:
+        one()
+    except emugemm.EmuGemmError:
+        failed += 1
+    try:
+        g.capture_end()
+    except RuntimeError:
+        failed += 1
+assert failed == 3, failed
+y.zero_()
+torch.cuda.synchronize()
+one()                                          # raised what the capture's call had already reported
+h.sync()
+xd = x.double().cpu().numpy()
+ref = xd @ w[0].T
+assert (abs(y.double().cpu().numpy() - ref) <= q4ref.product_bound(xd, w[0], ref, group, "bf16")).all()
+print("right", flush=True)
+os._exit(0)
+"""
+    here = os.path.dirname(os.path.abspath(__file__))
+    path = os.pathsep.join([here, os.path.dirname(os.path.abspath(emugemm.__file__)), os.environ.get("PYTHONPATH", "")])
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": path}, capture_output=True, text=True,
+                       timeout=120)
+    assert r.returncode == 0 and "right" in r.stdout, r.stderr[-2000:]
