@@ -28,6 +28,7 @@ TC_KERNEL_CODES = {"auto": 0, "single": 1, "pair": 2, "fused": 3, "fusea": 4}
 F32, F16, BF16 = 0, 1, 2
 DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
 
+INVALID_SIZE = 4
 STATUS = {
     0: "SUCCESS", 1: "INVALID_HANDLE", 2: "NOT_IMPLEMENTED", 3: "INVALID_POINTER", 4: "INVALID_SIZE",
     5: "MEMORY_ERROR", 6: "INTERNAL_ERROR", 11: "INVALID_VALUE", 100: "ARCH_MISMATCH", 101: "TIMEOUT",
@@ -206,7 +207,16 @@ def _dtype(dtype, *xs) -> int:
 
 def q4_bytes(E: int, N: int, K: int, group: int) -> int:
     """Bytes of the packed 4-bit weights of E experts of N x K (emugemm_q4_bytes); 0 when a size is out of range."""
+    if (E | N | group) >> 31:           # negative, or ctypes would pass the low 32 bits on
+        return 0
     return int(lib().emugemm_q4_bytes(E, N, K, group))
+
+
+def _int32(fn: str, *sizes) -> None:
+    """INVALID_SIZE for a size that a C int does not hold, of which ctypes would pass the low 32 bits on. Calls ask first
+    whether (a | b | ...) >> 31 is 0, which takes 0.1 us against 0.9; sizes below 0 are refused by the library."""
+    if any(not -(1 << 31) <= n < 1 << 31 for n in sizes):
+        raise EmuGemmError(fn, INVALID_SIZE)
 
 
 def check(fn: str, code: int) -> None:
@@ -423,44 +433,60 @@ class Handle:
     # ---- 4-bit weights and expert routing (dtype: from the tensors, or emugemm.F32 / F16 / BF16 for raw pointers) ----
     def q4_pack(self, E, N, K, W, ldw, group, packed, dtype=None) -> None:
         """Quantise E * N rows of K weights into `packed` (q4_bytes(E, N, K, group) bytes)."""
+        if (E | N | group) >> 31:
+            _int32("emugemm_q4_pack", E, N, group)
         check("emugemm_q4_pack", lib().emugemm_q4_pack(self.h, E, N, K, self._at(W), ldw, _dtype(dtype, W), group,
                                                        self._at(packed)))
 
     def q4_unpack(self, E, N, K, group, packed, W, ldw) -> None:
         """The FP32 values of packed weights."""
+        if (E | N | group) >> 31:
+            _int32("emugemm_q4_unpack", E, N, group)
         check("emugemm_q4_unpack", lib().emugemm_q4_unpack(self.h, E, N, K, group, self._at(packed),
                                                            self._at(W, "torch.float32"), ldw))
 
     def q4_gemm(self, M, N, K, A, lda, packed, group, C, ldc, dtype=None) -> None:
         """C (M x N) = A (M x K) * W^T with packed 4-bit weights."""
+        if (M | N | group) >> 31:
+            _int32("emugemm_q4_gemm", M, N, group)
         check("emugemm_q4_gemm", lib().emugemm_q4_gemm(self.h, M, N, K, self._at(A), lda, _dtype(dtype, A, C), self._at(packed),
                                                        group, self._at(C), ldc))
 
     def q4_gemm_experts(self, R, E, N, K, A, lda, offsets, packed, group, C, ldc, dtype=None) -> None:
         """q4_gemm with weights of E experts over rows sorted by expert (offsets: E + 1 int32 on the device)."""
+        if (R | E | N | group) >> 31:
+            _int32("emugemm_q4_gemm_experts", R, E, N, group)
         check("emugemm_q4_gemm_experts",
               lib().emugemm_q4_gemm_experts(self.h, R, E, N, K, self._at(A), lda, _dtype(dtype, A, C),
                                             self._at(offsets, "torch.int32"), self._at(packed), group, self._at(C), ldc))
 
     def expert_sort(self, T, topk, E, expert, order, place, offsets) -> None:
         """Stable sort of T x topk expert ids; all arrays int32."""
+        if (T | topk | E) >> 31:
+            _int32("emugemm_expert_sort", T, topk, E)
         i = "torch.int32"
         check("emugemm_expert_sort", lib().emugemm_expert_sort(self.h, T, topk, E, self._at(expert, i), self._at(order, i),
                                                                self._at(place, i), self._at(offsets, i)))
 
     def expert_gather(self, T, topk, H, X, ldx, place, XS, ldxs, dtype=None) -> None:
         """XS[place[t, j]] = X[t]."""
+        if (T | topk | H) >> 31:
+            _int32("emugemm_expert_gather", T, topk, H)
         check("emugemm_expert_gather", lib().emugemm_expert_gather(self.h, T, topk, H, self._at(X), ldx, _dtype(dtype, X, XS),
                                                                    self._at(place, "torch.int32"), self._at(XS), ldxs))
 
     def expert_gather_backward(self, T, topk, H, dXS, lddxs, place, dX, lddx, dtype=None) -> None:
         """dX[t] = sum over j of dXS[place[t, j]]."""
+        if (T | topk | H) >> 31:
+            _int32("emugemm_expert_gather_backward", T, topk, H)
         check("emugemm_expert_gather_backward",
               lib().emugemm_expert_gather_backward(self.h, T, topk, H, self._at(dXS), lddxs, _dtype(dtype, dXS, dX),
                                                    self._at(place, "torch.int32"), self._at(dX), lddx))
 
     def expert_combine(self, T, topk, H, YS, ldys, place, weights, Y, ldy, dtype=None) -> None:
         """Y[t] = sum over j of weights[t, j] * YS[place[t, j]] (weights float32)."""
+        if (T | topk | H) >> 31:
+            _int32("emugemm_expert_combine", T, topk, H)
         check("emugemm_expert_combine",
               lib().emugemm_expert_combine(self.h, T, topk, H, self._at(YS), ldys, _dtype(dtype, YS, Y),
                                            self._at(place, "torch.int32"), self._at(weights, "torch.float32"), self._at(Y), ldy))
@@ -468,6 +494,8 @@ class Handle:
     def expert_combine_backward(self, T, topk, H, dY, lddy, YS, ldys, place, weights, dYS, lddys, dweights,
                                 dtype=None) -> None:
         """dYS[place[t, j]] = weights[t, j] * dY[t] and dweights[t, j] = <dY[t], YS[place[t, j]]>."""
+        if (T | topk | H) >> 31:
+            _int32("emugemm_expert_combine_backward", T, topk, H)
         f = "torch.float32"
         check("emugemm_expert_combine_backward",
               lib().emugemm_expert_combine_backward(self.h, T, topk, H, self._at(dY), lddy, self._at(YS), ldys,
