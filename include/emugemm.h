@@ -293,10 +293,11 @@ void emugemm_test_stall_next_launches(int n);
    handle's stream and can be captured into CUDA graphs. Only products of many rows use the handle's workspace, for rows of
    A that a tile load cannot read in place (FP32, or 16-bit rows not on 16-byte boundaries): such a call returns
    MEMORY_ERROR while capturing unless one of its size ran before, what a captured graph uses stays until the handle is
-   destroyed, and calls and replays of one handle must be ordered on the GPU, as all its calls. Sums are FP32 in a fixed
-   order (no atomics): the same call gives the same bits. A device-side wait that gave up is reported by emugemm_sync
-   (TIMEOUT). Status: INVALID_VALUE for an unknown dtype or group, INVALID_SIZE for a size or
-   leading dimension out of range, INVALID_POINTER for a null or misaligned pointer (elements by their size, packed
+   destroyed, and calls and replays of one handle must be ordered on the GPU, as all its calls. How many rows are many goes
+   by the type, the group and the size of the weights; up to 32 rows (16 in FP32; of experts R / min(E, R) rows, rounded
+   down) never are. Sums are FP32 in a fixed order (no atomics): the same call gives the same bits. A device-side wait that
+   gave up is reported by emugemm_sync (TIMEOUT). Status: INVALID_VALUE for an unknown dtype or group, INVALID_SIZE for a
+   size or leading dimension out of range, INVALID_POINTER for a null or misaligned pointer (elements by their size, packed
    weights by 16 bytes). Device-side indices (offsets, place) are bounds-checked by the kernels: a bad one touches no
    memory outside the given matrices. */
 typedef enum { EMU_DTYPE_F32 = 0, EMU_DTYPE_F16 = 1, EMU_DTYPE_BF16 = 2 } emu_dtype_t;

@@ -312,3 +312,55 @@ os._exit(0)
     r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": path}, capture_output=True, text=True,
                        timeout=120)
     assert r.returncode == 0 and "right" in r.stdout, r.stderr[-2000:]
+
+
+# ------------------------------------------------------------------------------------------- what needs no earlier run
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("kind,rows,many", [("bf16", 32, 100), ("fp16", 32, 100), ("fp32", 16, 40)])
+@pytest.mark.parametrize("E", [1, 3])
+def test_captures_within_the_documented_limit(cuda, group, kind, rows, many, E):
+    """Unaligned rows, a first call of the handle inside a capture: up to 32 rows (16 in FP32), of experts on the average, it
+    is captured and replays to the bits of an eager call; more rows are refused and can be captured after one call of the size."""
+    torch = cuda
+    N, K = 4096 // E, 8195
+    packed = torch.randint(0, 256, (emugemm.q4_bytes(E, N, K, group),), dtype=torch.uint8, device="cuda")
+    codes = E * -(-N // 16) * -(-K // 64) * 512
+    at = -(-codes // 256) * 256
+    packed[at:] = torch.full(((packed.numel() - at) // 2,), 0.01, dtype=torch.bfloat16, device="cuda").view(torch.uint8)
+    st = torch.cuda.Stream()
+    with emugemm.Handle(st) as h, torch.cuda.stream(st):
+        for per, fits in ((rows, True), (many, False)):
+            R = per * E + (E - 1 if fits else 0)
+            a = torch.randn(R, K, generator=torch.Generator().manual_seed(R)).to(TYPES[kind]).cuda()
+            off = torch.arange(0, (per + 1) * E, per, dtype=torch.int32, device="cuda")
+            off[E] = R
+            c = torch.zeros(R, N, dtype=TYPES[kind], device="cuda")
+
+            def call():
+                if E == 1:
+                    h.q4_gemm(R, N, K, a, K, packed, group, c, N)
+                else:
+                    h.q4_gemm_experts(R, E, N, K, a, K, off, packed, group, c, N)
+
+            torch.cuda.synchronize()
+            if not fits:
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=st):
+                    with pytest.raises(emugemm.EmuGemmError) as e:
+                        call()
+                    assert e.value.code == 5        # MEMORY_ERROR
+                    c.add_(1)
+                call()
+                torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=st):
+                call()
+            c.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            got = c.clone()
+            c.zero_()
+            call()
+            h.sync()
+            assert torch.equal(got, c) and c.abs().sum() > 0
+            del graph
