@@ -310,7 +310,8 @@ typedef enum { EMU_DTYPE_F32 = 0, EMU_DTYPE_F16 = 1, EMU_DTYPE_BF16 = 2 } emu_dt
        bytes, ordered [expert][row block][k block]; bytes (4g + t) * 16 .. + 15 of a tile (g = 0..7, t = 0..3) are four
        32-bit words: row g at k = 8t..8t+7, row g + 8 at the same k, row g at k = 32 + 8t.., row g + 8 at the same; in a
        word k = 0, 2, 4, 6, 1, 3, 5, 7 take the nibbles from the lowest up;
-     scales: at the next multiple of 256 bytes, bf16 [expert][row block][group][8][2], rows g and g + 8 side by side. */
+     scales: at the next multiple of 256 bytes, bf16 [expert][row block][group][8][2], rows g and g + 8 side by side; finite,
+       or NaN for a group that reads as NaN (a product with an infinite scale may be NaN). */
 size_t emugemm_q4_bytes(int E, int N, long K, int group);
 /* Quantises W (E * N rows of K values, ldw >= K; a linear layer's weights, one row per output) into `packed`. Per group
    scale = bf16(fp32(max|w| / 7)), q = w / scale rounded to the nearest integer (ties to even, decided exactly) and kept
