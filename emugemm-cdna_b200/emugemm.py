@@ -414,9 +414,10 @@ class Handle:
     def split_f16(self, X, n, hi, lo) -> None:
         check("emugemm_split_f16", lib().emugemm_split_f16(self.h, _ptr(X), n, _ptr(hi), _ptr(lo)))
 
-    def _at(self, x, name: str | None = None) -> int:
-        """Address of x (None, an address, or a tensor). A tensor must be on the handle's device and, with `name`, have that
-        dtype (ValueError): a kernel given a host address or another type's bytes would fault or compute nonsense."""
+    def _at(self, x, name: str | None = None, n: int = 0) -> int:
+        """Address of x (None, an address, or a tensor). A tensor must be on the handle's device, with `name` have that dtype,
+        and with `n` (an array that has no leading dimension) hold n values one behind the other (ValueError): a kernel
+        given a host address, another type's bytes, gaps or too few values would fault or compute nonsense."""
         if x is None or isinstance(x, int):
             return x or 0
         if x.get_device() != self.device:
@@ -428,6 +429,8 @@ class Handle:
                 known = _dtype_names[d] = str(d)
             if known != name:
                 raise ValueError(f"expected a {name} tensor, got {d}")
+            if n and not (x.numel() >= n and x.is_contiguous()):
+                raise ValueError(f"expected {n} contiguous values, got shape {tuple(x.shape)}, strides {x.stride()}")
         return x.data_ptr()
 
     # ---- 4-bit weights and expert routing (dtype: from the tensors, or emugemm.F32 / F16 / BF16 for raw pointers) ----
@@ -458,22 +461,23 @@ class Handle:
             _int32("emugemm_q4_gemm_experts", R, E, N, group)
         check("emugemm_q4_gemm_experts",
               lib().emugemm_q4_gemm_experts(self.h, R, E, N, K, self._at(A), lda, _dtype(dtype, A, C),
-                                            self._at(offsets, "torch.int32"), self._at(packed), group, self._at(C), ldc))
+                                            self._at(offsets, "torch.int32", E + 1), self._at(packed), group, self._at(C), ldc))
 
     def expert_sort(self, T, topk, E, expert, order, place, offsets) -> None:
         """Stable sort of T x topk expert ids; all arrays int32."""
         if (T | topk | E) >> 31:
             _int32("emugemm_expert_sort", T, topk, E)
         i = "torch.int32"
-        check("emugemm_expert_sort", lib().emugemm_expert_sort(self.h, T, topk, E, self._at(expert, i), self._at(order, i),
-                                                               self._at(place, i), self._at(offsets, i)))
+        check("emugemm_expert_sort", lib().emugemm_expert_sort(self.h, T, topk, E, self._at(expert, i, T * topk),
+                                                               self._at(order, i, T * topk), self._at(place, i, T * topk),
+                                                               self._at(offsets, i, E + 1)))
 
     def expert_gather(self, T, topk, H, X, ldx, place, XS, ldxs, dtype=None) -> None:
         """XS[place[t, j]] = X[t]."""
         if (T | topk | H) >> 31:
             _int32("emugemm_expert_gather", T, topk, H)
         check("emugemm_expert_gather", lib().emugemm_expert_gather(self.h, T, topk, H, self._at(X), ldx, _dtype(dtype, X, XS),
-                                                                   self._at(place, "torch.int32"), self._at(XS), ldxs))
+                                                                   self._at(place, "torch.int32", T * topk), self._at(XS), ldxs))
 
     def expert_gather_backward(self, T, topk, H, dXS, lddxs, place, dX, lddx, dtype=None) -> None:
         """dX[t] = sum over j of dXS[place[t, j]]."""
@@ -481,7 +485,7 @@ class Handle:
             _int32("emugemm_expert_gather_backward", T, topk, H)
         check("emugemm_expert_gather_backward",
               lib().emugemm_expert_gather_backward(self.h, T, topk, H, self._at(dXS), lddxs, _dtype(dtype, dXS, dX),
-                                                   self._at(place, "torch.int32"), self._at(dX), lddx))
+                                                   self._at(place, "torch.int32", T * topk), self._at(dX), lddx))
 
     def expert_combine(self, T, topk, H, YS, ldys, place, weights, Y, ldy, dtype=None) -> None:
         """Y[t] = sum over j of weights[t, j] * YS[place[t, j]] (weights float32)."""
@@ -489,7 +493,8 @@ class Handle:
             _int32("emugemm_expert_combine", T, topk, H)
         check("emugemm_expert_combine",
               lib().emugemm_expert_combine(self.h, T, topk, H, self._at(YS), ldys, _dtype(dtype, YS, Y),
-                                           self._at(place, "torch.int32"), self._at(weights, "torch.float32"), self._at(Y), ldy))
+                                           self._at(place, "torch.int32", T * topk),
+                                           self._at(weights, "torch.float32", T * topk), self._at(Y), ldy))
 
     def expert_combine_backward(self, T, topk, H, dY, lddy, YS, ldys, place, weights, dYS, lddys, dweights,
                                 dtype=None) -> None:
@@ -499,8 +504,9 @@ class Handle:
         f = "torch.float32"
         check("emugemm_expert_combine_backward",
               lib().emugemm_expert_combine_backward(self.h, T, topk, H, self._at(dY), lddy, self._at(YS), ldys,
-                                                    _dtype(dtype, dY, YS, dYS), self._at(place, "torch.int32"),
-                                                    self._at(weights, f), self._at(dYS), lddys, self._at(dweights, f)))
+                                                    _dtype(dtype, dY, YS, dYS), self._at(place, "torch.int32", T * topk),
+                                                    self._at(weights, f, T * topk), self._at(dYS), lddys,
+                                                    self._at(dweights, f, T * topk)))
 
     PROF_KINDS = ["tc_gemm", "fp32_gemm", "split", "scan", "rho", "reduce", "q4", "expert"]
 
