@@ -190,8 +190,9 @@ _dtype_names: dict = {}   # tensor dtype -> its name (str of a dtype takes longe
 def _dtype(dtype, *xs) -> int:
     """emu_dtype_t of the operands: the given code, or that of the tensors, which must agree (ValueError)."""
     for x in xs:
-        d = getattr(x, "dtype", None)
-        if d is None:
+        try:
+            d = x.dtype
+        except AttributeError:
             continue
         code = _dtype_codes.get(d)
         if code is None:
@@ -205,6 +206,20 @@ def _dtype(dtype, *xs) -> int:
     return dtype
 
 
+_dtype_pairs: dict = {}   # (given code or None, dtype, dtype) -> emu_dtype_t, of those that _dtype has accepted
+
+
+def _dtype2(dtype, x, y) -> int:
+    """_dtype of two operands (in half the time)."""
+    try:
+        return _dtype_pairs[dtype, x.dtype, y.dtype]
+    except (AttributeError, KeyError):
+        code = _dtype(dtype, x, y)
+        if hasattr(x, "dtype") and hasattr(y, "dtype"):
+            _dtype_pairs[dtype, x.dtype, y.dtype] = code
+        return code
+
+
 def q4_bytes(E: int, N: int, K: int, group: int) -> int:
     """Bytes of the packed 4-bit weights of E experts of N x K (emugemm_q4_bytes); 0 when a size is out of range."""
     if (E | N | group) >> 31:           # negative, or ctypes would pass the low 32 bits on
@@ -214,7 +229,7 @@ def q4_bytes(E: int, N: int, K: int, group: int) -> int:
 
 def _int32(fn: str, *sizes) -> None:
     """INVALID_SIZE for a size that a C int does not hold, of which ctypes would pass the low 32 bits on. Calls ask first
-    whether (a | b | ...) >> 31 is 0, which takes 0.1 us against 0.9; sizes below 0 are refused by the library."""
+    whether (a | b | ...) >> 31 is 0, which takes a ninth of the time; sizes below 0 are refused by the library."""
     if any(not -(1 << 31) <= n < 1 << 31 for n in sizes):
         raise EmuGemmError(fn, INVALID_SIZE)
 
@@ -414,99 +429,114 @@ class Handle:
     def split_f16(self, X, n, hi, lo) -> None:
         check("emugemm_split_f16", lib().emugemm_split_f16(self.h, _ptr(X), n, _ptr(hi), _ptr(lo)))
 
-    def _at(self, x, name: str | None = None, n: int = 0) -> int:
-        """Address of x (None, an address, or a tensor). A tensor must be on the handle's device, with `name` have that dtype,
-        and with `n` (an array that has no leading dimension) hold n values one behind the other (ValueError): a kernel
-        given a host address, another type's bytes, gaps or too few values would fault or compute nonsense."""
-        if x is None or isinstance(x, int):
+    def _at(self, x, name: str | None = None, nbytes: int = 0) -> int:
+        """Address of x (None, an address, or a tensor). A tensor must be on the handle's device, with `name` have that
+        dtype, and with `nbytes` (an array that has no leading dimension) hold so many bytes one behind the other
+        (ValueError): a kernel given a host address, another type's bytes, gaps or too few values would fault or compute
+        nonsense."""
+        try:
+            device = x.get_device()
+        except AttributeError:
             return x or 0
-        if x.get_device() != self.device:
+        if device != self.device:
             raise ValueError(f"expected a tensor on cuda:{self.device}, got one on {x.device}")
-        if name is not None:
-            d = x.dtype
-            known = _dtype_names.get(d)
-            if known is None:
-                known = _dtype_names[d] = str(d)
-            if known != name:
-                raise ValueError(f"expected a {name} tensor, got {d}")
-            if n and not (x.numel() >= n and x.is_contiguous()):
-                raise ValueError(f"expected {n} contiguous values, got shape {tuple(x.shape)}, strides {x.stride()}")
+        if name is not None and _dtype_names.get(x.dtype) != name and _dtype_names.setdefault(x.dtype, str(x.dtype)) != name:
+            raise ValueError(f"expected a {name} tensor, got {x.dtype}")
+        if nbytes and not (x.nbytes >= nbytes and x.is_contiguous()):
+            raise ValueError(f"expected {nbytes} bytes without gaps, got shape {tuple(x.shape)}, strides {x.stride()}")
         return x.data_ptr()
 
     # ---- 4-bit weights and expert routing (dtype: from the tensors, or emugemm.F32 / F16 / BF16 for raw pointers) ----
+    # A call on few rows is host time, so these spell out lib() and check().
     def q4_pack(self, E, N, K, W, ldw, group, packed, dtype=None) -> None:
         """Quantise E * N rows of K weights into `packed` (q4_bytes(E, N, K, group) bytes)."""
         if (E | N | group) >> 31:
             _int32("emugemm_q4_pack", E, N, group)
-        check("emugemm_q4_pack", lib().emugemm_q4_pack(self.h, E, N, K, self._at(W), ldw, _dtype(dtype, W), group,
-                                                       self._at(packed)))
+        code = (_lib or lib()).emugemm_q4_pack(self.h, E, N, K, self._at(W), ldw, _dtype(dtype, W), group, self._at(packed))
+        if code:
+            raise EmuGemmError("emugemm_q4_pack", code)
 
     def q4_unpack(self, E, N, K, group, packed, W, ldw) -> None:
         """The FP32 values of packed weights."""
         if (E | N | group) >> 31:
             _int32("emugemm_q4_unpack", E, N, group)
-        check("emugemm_q4_unpack", lib().emugemm_q4_unpack(self.h, E, N, K, group, self._at(packed),
-                                                           self._at(W, "torch.float32"), ldw))
+        code = (_lib or lib()).emugemm_q4_unpack(self.h, E, N, K, group, self._at(packed), self._at(W, "torch.float32"), ldw)
+        if code:
+            raise EmuGemmError("emugemm_q4_unpack", code)
 
     def q4_gemm(self, M, N, K, A, lda, packed, group, C, ldc, dtype=None) -> None:
         """C (M x N) = A (M x K) * W^T with packed 4-bit weights."""
         if (M | N | group) >> 31:
             _int32("emugemm_q4_gemm", M, N, group)
-        check("emugemm_q4_gemm", lib().emugemm_q4_gemm(self.h, M, N, K, self._at(A), lda, _dtype(dtype, A, C), self._at(packed),
-                                                       group, self._at(C), ldc))
+        at = self._at
+        code = (_lib or lib()).emugemm_q4_gemm(self.h, M, N, K, at(A), lda, _dtype2(dtype, A, C),
+                                               at(packed), group, at(C), ldc)
+        if code:
+            raise EmuGemmError("emugemm_q4_gemm", code)
 
     def q4_gemm_experts(self, R, E, N, K, A, lda, offsets, packed, group, C, ldc, dtype=None) -> None:
         """q4_gemm with weights of E experts over rows sorted by expert (offsets: E + 1 int32 on the device)."""
         if (R | E | N | group) >> 31:
             _int32("emugemm_q4_gemm_experts", R, E, N, group)
-        check("emugemm_q4_gemm_experts",
-              lib().emugemm_q4_gemm_experts(self.h, R, E, N, K, self._at(A), lda, _dtype(dtype, A, C),
-                                            self._at(offsets, "torch.int32", E + 1), self._at(packed), group, self._at(C), ldc))
+        at = self._at
+        code = (_lib or lib()).emugemm_q4_gemm_experts(self.h, R, E, N, K, at(A), lda, _dtype2(dtype, A, C),
+                                                       at(offsets, "torch.int32", 4 * E + 4), at(packed), group,
+                                                       at(C), ldc)
+        if code:
+            raise EmuGemmError("emugemm_q4_gemm_experts", code)
 
     def expert_sort(self, T, topk, E, expert, order, place, offsets) -> None:
         """Stable sort of T x topk expert ids; all arrays int32."""
         if (T | topk | E) >> 31:
             _int32("emugemm_expert_sort", T, topk, E)
-        i = "torch.int32"
-        check("emugemm_expert_sort", lib().emugemm_expert_sort(self.h, T, topk, E, self._at(expert, i, T * topk),
-                                                               self._at(order, i, T * topk), self._at(place, i, T * topk),
-                                                               self._at(offsets, i, E + 1)))
+        at, i, n = self._at, "torch.int32", 4 * T * topk
+        code = (_lib or lib()).emugemm_expert_sort(self.h, T, topk, E, at(expert, i, n), at(order, i, n),
+                                                   at(place, i, n), at(offsets, i, 4 * E + 4))
+        if code:
+            raise EmuGemmError("emugemm_expert_sort", code)
 
     def expert_gather(self, T, topk, H, X, ldx, place, XS, ldxs, dtype=None) -> None:
         """XS[place[t, j]] = X[t]."""
         if (T | topk | H) >> 31:
             _int32("emugemm_expert_gather", T, topk, H)
-        check("emugemm_expert_gather", lib().emugemm_expert_gather(self.h, T, topk, H, self._at(X), ldx, _dtype(dtype, X, XS),
-                                                                   self._at(place, "torch.int32", T * topk), self._at(XS), ldxs))
+        at = self._at
+        code = (_lib or lib()).emugemm_expert_gather(self.h, T, topk, H, at(X), ldx, _dtype2(dtype, X, XS),
+                                                     at(place, "torch.int32", 4 * T * topk), at(XS), ldxs)
+        if code:
+            raise EmuGemmError("emugemm_expert_gather", code)
 
     def expert_gather_backward(self, T, topk, H, dXS, lddxs, place, dX, lddx, dtype=None) -> None:
         """dX[t] = sum over j of dXS[place[t, j]]."""
         if (T | topk | H) >> 31:
             _int32("emugemm_expert_gather_backward", T, topk, H)
-        check("emugemm_expert_gather_backward",
-              lib().emugemm_expert_gather_backward(self.h, T, topk, H, self._at(dXS), lddxs, _dtype(dtype, dXS, dX),
-                                                   self._at(place, "torch.int32", T * topk), self._at(dX), lddx))
+        at = self._at
+        code = (_lib or lib()).emugemm_expert_gather_backward(self.h, T, topk, H, at(dXS), lddxs, _dtype2(dtype, dXS, dX),
+                                                              at(place, "torch.int32", 4 * T * topk), at(dX), lddx)
+        if code:
+            raise EmuGemmError("emugemm_expert_gather_backward", code)
 
     def expert_combine(self, T, topk, H, YS, ldys, place, weights, Y, ldy, dtype=None) -> None:
         """Y[t] = sum over j of weights[t, j] * YS[place[t, j]] (weights float32)."""
         if (T | topk | H) >> 31:
             _int32("emugemm_expert_combine", T, topk, H)
-        check("emugemm_expert_combine",
-              lib().emugemm_expert_combine(self.h, T, topk, H, self._at(YS), ldys, _dtype(dtype, YS, Y),
-                                           self._at(place, "torch.int32", T * topk),
-                                           self._at(weights, "torch.float32", T * topk), self._at(Y), ldy))
+        at, n = self._at, 4 * T * topk
+        code = (_lib or lib()).emugemm_expert_combine(self.h, T, topk, H, at(YS), ldys, _dtype2(dtype, YS, Y),
+                                                      at(place, "torch.int32", n), at(weights, "torch.float32", n),
+                                                      at(Y), ldy)
+        if code:
+            raise EmuGemmError("emugemm_expert_combine", code)
 
     def expert_combine_backward(self, T, topk, H, dY, lddy, YS, ldys, place, weights, dYS, lddys, dweights,
                                 dtype=None) -> None:
         """dYS[place[t, j]] = weights[t, j] * dY[t] and dweights[t, j] = <dY[t], YS[place[t, j]]>."""
         if (T | topk | H) >> 31:
             _int32("emugemm_expert_combine_backward", T, topk, H)
-        f = "torch.float32"
-        check("emugemm_expert_combine_backward",
-              lib().emugemm_expert_combine_backward(self.h, T, topk, H, self._at(dY), lddy, self._at(YS), ldys,
-                                                    _dtype(dtype, dY, YS, dYS), self._at(place, "torch.int32", T * topk),
-                                                    self._at(weights, f, T * topk), self._at(dYS), lddys,
-                                                    self._at(dweights, f, T * topk)))
+        at, f, n = self._at, "torch.float32", 4 * T * topk
+        code = (_lib or lib()).emugemm_expert_combine_backward(self.h, T, topk, H, at(dY), lddy, at(YS), ldys,
+                                                               _dtype(dtype, dY, YS, dYS), at(place, "torch.int32", n),
+                                                               at(weights, f, n), at(dYS), lddys, at(dweights, f, n))
+        if code:
+            raise EmuGemmError("emugemm_expert_combine_backward", code)
 
     PROF_KINDS = ["tc_gemm", "fp32_gemm", "split", "scan", "rho", "reduce", "q4", "expert"]
 

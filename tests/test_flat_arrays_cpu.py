@@ -37,7 +37,7 @@ CALLS = {
 
 @pytest.mark.parametrize("name,arg", [(n, a) for n, (_, args) in CALLS.items() for a in args])
 def test_gaps_and_too_few_values_are_refused(monkeypatch, name, arg):
-    monkeypatch.setattr(emugemm, "lib", lambda: StandIn())
+    monkeypatch.setattr(emugemm, "_lib", StandIn())
     h = emugemm.Handle.__new__(emugemm.Handle)
     h.h, h.device = None, -1                        # -1: the host, where these tensors are
     kw, sizes = CALLS[name]
@@ -53,7 +53,7 @@ def test_gaps_and_too_few_values_are_refused(monkeypatch, name, arg):
 
 
 def test_no_tokens_need_no_arrays(monkeypatch):
-    monkeypatch.setattr(emugemm, "lib", lambda: StandIn())
+    monkeypatch.setattr(emugemm, "_lib", StandIn())
     h = emugemm.Handle.__new__(emugemm.Handle)
     h.h, h.device = None, -1
     h.expert_sort(0, 2, 5, None, None, None, i32(6))

@@ -28,7 +28,7 @@ class StandIn:
 @pytest.fixture()
 def library(monkeypatch):
     lib = StandIn()
-    monkeypatch.setattr(emugemm, "lib", lambda: lib)
+    monkeypatch.setattr(emugemm, "_lib", lib)
 
 
 def test_handle_beside_a_torch_without_cuda(library, monkeypatch):

@@ -34,7 +34,7 @@ class StandIn:
 @pytest.mark.parametrize("name", list(OK))
 def test_calls_refuse_sizes_beyond_int(monkeypatch, name):
     lib = StandIn()
-    monkeypatch.setattr(emugemm, "lib", lambda: lib)
+    monkeypatch.setattr(emugemm, "_lib", lib)
     h = emugemm.Handle.__new__(emugemm.Handle)
     h.h, h.device = None, 0
     kw, sizes = OK[name]
