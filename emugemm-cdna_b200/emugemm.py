@@ -11,6 +11,7 @@ import ctypes
 import os
 import pathlib
 import re
+import sys
 
 HERE = pathlib.Path(__file__).resolve().parent
 LIB_PATH = HERE / "libemugemm.so"
@@ -184,7 +185,15 @@ def _ptr(x) -> int:
 
 
 _dtype_codes: dict = {}   # tensor dtype -> emu_dtype_t
-_dtype_names: dict = {}   # tensor dtype -> its name (str of a dtype takes longer than the rest of a call's checks)
+# torch's types of the index and weight arrays (their names until a call has seen a tensor: torch need not be there). A
+# comparison with `is` costs a call less host time than one of names.
+_i32, _f32 = "torch.int32", "torch.float32"
+
+
+def _torch_types() -> None:
+    global _i32, _f32
+    torch = sys.modules["torch"]
+    _i32, _f32 = torch.int32, torch.float32
 
 
 def _dtype(dtype, *xs) -> int:
@@ -429,21 +438,31 @@ class Handle:
     def split_f16(self, X, n, hi, lo) -> None:
         check("emugemm_split_f16", lib().emugemm_split_f16(self.h, _ptr(X), n, _ptr(hi), _ptr(lo)))
 
-    def _at(self, x, name: str | None = None, nbytes: int = 0) -> int:
-        """Address of x (None, an address, or a tensor). A tensor must be on the handle's device, with `name` have that
-        dtype, and with `nbytes` (an array that has no leading dimension) hold so many bytes one behind the other
-        (ValueError): a kernel given a host address, another type's bytes, gaps or too few values would fault or compute
-        nonsense."""
+    def _at(self, x, name: str | None = None) -> int:
+        """Address of x (None, an address, or a tensor). A tensor must be on the handle's device and, with `name`, have that
+        dtype (ValueError): a kernel given a host address or another type's bytes would fault or compute nonsense."""
         try:
             device = x.get_device()
         except AttributeError:
             return x or 0
         if device != self.device:
             raise ValueError(f"expected a tensor on cuda:{self.device}, got one on {x.device}")
-        if name is not None and _dtype_names.get(x.dtype) != name and _dtype_names.setdefault(x.dtype, str(x.dtype)) != name:
+        if name is not None and str(x.dtype) != name:
             raise ValueError(f"expected a {name} tensor, got {x.dtype}")
-        if nbytes and not (x.nbytes >= nbytes and x.is_contiguous()):
-            raise ValueError(f"expected {nbytes} bytes without gaps, got shape {tuple(x.shape)}, strides {x.stride()}")
+        return x.data_ptr()
+
+    def _flat(self, x, t) -> int:
+        """_at of an array without a leading dimension, which kernels take without gaps. t: _i32 or _f32, or before torch's
+        types are known their name."""
+        try:
+            device = x.get_device()
+        except AttributeError:
+            return x or 0
+        if device != self.device or x.dtype is not t or not x.is_contiguous():
+            self._at(x, str(t))     # says which, if it is not the strides
+            if not x.is_contiguous():
+                raise ValueError(f"expected values without gaps, got shape {tuple(x.shape)}, strides {x.stride()}")
+            _torch_types()
         return x.data_ptr()
 
     # ---- 4-bit weights and expert routing (dtype: from the tensors, or emugemm.F32 / F16 / BF16 for raw pointers) ----
@@ -480,8 +499,7 @@ class Handle:
             _int32("emugemm_q4_gemm_experts", R, E, N, group)
         at = self._at
         code = (_lib or lib()).emugemm_q4_gemm_experts(self.h, R, E, N, K, at(A), lda, _dtype2(dtype, A, C),
-                                                       at(offsets, "torch.int32", 4 * E + 4), at(packed), group,
-                                                       at(C), ldc)
+                                                       self._flat(offsets, _i32), at(packed), group, at(C), ldc)
         if code:
             raise EmuGemmError("emugemm_q4_gemm_experts", code)
 
@@ -489,9 +507,9 @@ class Handle:
         """Stable sort of T x topk expert ids; all arrays int32."""
         if (T | topk | E) >> 31:
             _int32("emugemm_expert_sort", T, topk, E)
-        at, i, n = self._at, "torch.int32", 4 * T * topk
-        code = (_lib or lib()).emugemm_expert_sort(self.h, T, topk, E, at(expert, i, n), at(order, i, n),
-                                                   at(place, i, n), at(offsets, i, 4 * E + 4))
+        flat, i = self._flat, _i32
+        code = (_lib or lib()).emugemm_expert_sort(self.h, T, topk, E, flat(expert, i), flat(order, i),
+                                                   flat(place, i), flat(offsets, i))
         if code:
             raise EmuGemmError("emugemm_expert_sort", code)
 
@@ -501,7 +519,7 @@ class Handle:
             _int32("emugemm_expert_gather", T, topk, H)
         at = self._at
         code = (_lib or lib()).emugemm_expert_gather(self.h, T, topk, H, at(X), ldx, _dtype2(dtype, X, XS),
-                                                     at(place, "torch.int32", 4 * T * topk), at(XS), ldxs)
+                                                     self._flat(place, _i32), at(XS), ldxs)
         if code:
             raise EmuGemmError("emugemm_expert_gather", code)
 
@@ -511,7 +529,7 @@ class Handle:
             _int32("emugemm_expert_gather_backward", T, topk, H)
         at = self._at
         code = (_lib or lib()).emugemm_expert_gather_backward(self.h, T, topk, H, at(dXS), lddxs, _dtype2(dtype, dXS, dX),
-                                                              at(place, "torch.int32", 4 * T * topk), at(dX), lddx)
+                                                              self._flat(place, _i32), at(dX), lddx)
         if code:
             raise EmuGemmError("emugemm_expert_gather_backward", code)
 
@@ -519,10 +537,9 @@ class Handle:
         """Y[t] = sum over j of weights[t, j] * YS[place[t, j]] (weights float32)."""
         if (T | topk | H) >> 31:
             _int32("emugemm_expert_combine", T, topk, H)
-        at, n = self._at, 4 * T * topk
+        at, flat = self._at, self._flat
         code = (_lib or lib()).emugemm_expert_combine(self.h, T, topk, H, at(YS), ldys, _dtype2(dtype, YS, Y),
-                                                      at(place, "torch.int32", n), at(weights, "torch.float32", n),
-                                                      at(Y), ldy)
+                                                      flat(place, _i32), flat(weights, _f32), at(Y), ldy)
         if code:
             raise EmuGemmError("emugemm_expert_combine", code)
 
@@ -531,10 +548,10 @@ class Handle:
         """dYS[place[t, j]] = weights[t, j] * dY[t] and dweights[t, j] = <dY[t], YS[place[t, j]]>."""
         if (T | topk | H) >> 31:
             _int32("emugemm_expert_combine_backward", T, topk, H)
-        at, f, n = self._at, "torch.float32", 4 * T * topk
+        at, flat = self._at, self._flat
         code = (_lib or lib()).emugemm_expert_combine_backward(self.h, T, topk, H, at(dY), lddy, at(YS), ldys,
-                                                               _dtype(dtype, dY, YS, dYS), at(place, "torch.int32", n),
-                                                               at(weights, f, n), at(dYS), lddys, at(dweights, f, n))
+                                                               _dtype(dtype, dY, YS, dYS), flat(place, _i32),
+                                                               flat(weights, _f32), at(dYS), lddys, flat(dweights, _f32))
         if code:
             raise EmuGemmError("emugemm_expert_combine_backward", code)
 

@@ -1,5 +1,5 @@
 """Arrays without a leading dimension (ids, places, offsets, weights of the choices) are refused when a tensor does not hold
-their values one behind the other; host tensors stand in for device ones, and nothing is launched."""
+its values one behind the other; host tensors stand in for device ones, and nothing is launched."""
 from __future__ import annotations
 
 import pytest
@@ -36,7 +36,7 @@ CALLS = {
 
 
 @pytest.mark.parametrize("name,arg", [(n, a) for n, (_, args) in CALLS.items() for a in args])
-def test_gaps_and_too_few_values_are_refused(monkeypatch, name, arg):
+def test_gaps_are_refused(monkeypatch, name, arg):
     monkeypatch.setattr(emugemm, "_lib", StandIn())
     h = emugemm.Handle.__new__(emugemm.Handle)
     h.h, h.device = None, -1                        # -1: the host, where these tensors are
@@ -46,8 +46,9 @@ def test_gaps_and_too_few_values_are_refused(monkeypatch, name, arg):
     call(**kw)
     call(**{**kw, arg: P})                          # an address is taken as it is
     call(**{**kw, arg: torch.zeros(n + 3, dtype=t)[1:]})
+    other = torch.float64 if t == torch.float32 else torch.int64
     for bad in (torch.zeros(2 * n, dtype=t)[::2], torch.zeros(TOPK, n, dtype=t).t(), torch.zeros(1, dtype=t).expand(n),
-                torch.zeros(n - 1, dtype=t), torch.zeros(n, 3, dtype=t)[:, :2]):
+                torch.zeros(n, 3, dtype=t)[:, :2], torch.zeros(n, dtype=other)):
         with pytest.raises(ValueError):
             call(**{**kw, arg: bad})
 
@@ -58,3 +59,20 @@ def test_no_tokens_need_no_arrays(monkeypatch):
     h.h, h.device = None, -1
     h.expert_sort(0, 2, 5, None, None, None, i32(6))
     h.expert_gather(0, 2, 16, P, 16, i32(0, 2), P, 16, dtype=0)
+
+
+def test_types_before_and_after_the_first_tensor(monkeypatch):
+    """The names stand for torch's types until a call has seen a tensor."""
+    for name, t in (("_i32", torch.int32), ("_f32", torch.float32)):
+        monkeypatch.setattr(emugemm, name, str(t))
+    monkeypatch.setattr(emugemm, "_lib", StandIn())
+    h = emugemm.Handle.__new__(emugemm.Handle)
+    h.h, h.device = None, -1
+    kw, _ = CALLS["expert_combine"]
+    with pytest.raises(ValueError):
+        h.expert_combine(**{**kw, "weights": torch.zeros(T, TOPK, dtype=torch.int32)})
+    h.expert_combine(**kw)
+    assert emugemm._i32 is torch.int32 and emugemm._f32 is torch.float32
+    h.expert_combine(**kw)
+    with pytest.raises(ValueError):
+        h.expert_combine(**{**kw, "weights": torch.zeros(T, TOPK, dtype=torch.int32)})
