@@ -66,7 +66,8 @@ inline __host__ __device__ Layout layout(long E, long N, long K, int group) {
 // others, bounds the unpacking: 5 operations on it per word, against 7 with every nibble shifted to bit 0).
 //   bf16: the low byte u of a half is a subnormal or first-binade bf16, u * 2^-133 for all 256 values; one fused
 //         multiply-add by 2^127 (nibble at bit 0) or 2^123 (at bit 4) and minus 8 * 2^-6 gives q * 2^-6;
-//   fp16: the nibble as low mantissa bits of 1024: 1024 + u or 1024 + 16 u, minus 1032, or times 1/16 minus 72.
+//   fp16: the nibble as low mantissa bits of 1024: 1024 + u or 1024 + 16 u, minus 1032, or times 1/16 minus 72 (the
+//         conversion by an exponent's offset, as in Kim, Henry, Fahim and Awadalla, "Who Says Elephants Can't Run", 2022).
 template <bool BF16>
 __device__ __forceinline__ constexpr float code_unit() { return BF16 ? 64.f : 1.f; }
 template <bool BF16>

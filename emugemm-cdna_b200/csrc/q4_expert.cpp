@@ -45,7 +45,8 @@ emugemm_status_t q4_product(emugemm_handle_t handle, int R, int E, int N, long K
     a.err = h->err_dev;
     const int with = experts ? (E < R ? E : R) : 1;   // experts that can have rows
     const long cols = (long)(R / with) * (dtype == EMU_DTYPE_F32 ? 3 : 1);
-    // Few columns: one pass over the codes per 48 of them (k_q4.cu), else tiles of CTA pairs (k_q4_tc.cu), in us:
+    // Few columns: one pass over the codes per 48 of them (k_q4.cu; of experts by the mean, since the rows of each are known on
+    // the device only, and the passes of one expert follow one another), else tiles of CTA pairs (k_q4_tc.cu), in us:
     //   48 columns, groups of 128:  4096 x 4096 13.7 against 15.0, 8192 x 4096 20.3 / 19.0, 8192 x 8192 35.4 / 29.4
     //   32 columns, groups of 128:  8192 x 8192 26.1 / 28.8;  48 columns, groups of 64:  11008 x 4096 29.8 / 37.8
     //   16 rows FP32 (48 columns):  4096 x 4096 13.1 / 19.4;  64 columns, groups of 128:  4096 x 4096 23 / 15

@@ -1,7 +1,8 @@
-"""4-bit products on the GPU, what the other files leave of their range: workspaces that captured graphs keep, and row tiles
-of both heights with more tiles than CTA pairs.
+"""4-bit products on the GPU, what the other files leave of their range: workspaces that captured graphs keep, row tiles of
+both heights with more tiles than CTA pairs, the low bits of FP32 rows, rows that are not there, the choice between the
+kernels, captures without an earlier run, and the calls after a failed one.
 
-Bars: q4ref.product_bound."""
+Bars: q4ref.product_bound, or derived at the test."""
 from __future__ import annotations
 
 import functools
